@@ -267,6 +267,86 @@ int taco_debug_conv_gemm(const float* X, int32_t ldx, int32_t M, int32_t T, int3
                          const float* scale, const float* shift, const float* R, int32_t ldr, float* C,
                          int32_t ldc, int32_t act, int32_t pool, taco_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Paged key-value cache of an attention decoder (no counterpart in the reference, whose decoder attends one fixed
+ * memory per utterance: model/decoder.py:24-27). For decoders whose memories are long, ragged or grow while they decode:
+ * a pool of pages shared by all sequences, the attention of ONE new token per sequence over its pages (what taco_decode
+ * does once per step over the encoder outputs, as a scaled dot product with any number of query heads per key head), and
+ * an eviction that bounds a memory by the attention its tokens have drawn, summed over the steps (the alignments).
+ *
+ * No model handle: no weights take part. Unlike the calls above, tensors may be strided where a stride is an argument.
+ * Strides are in elements; every row of head_dim elements is contiguous and starts on a 16-byte boundary. Lengths, page
+ * ids and counts are device data and are never trusted: a length outside 0 .. max_pages * page_size is clamped, a slot
+ * whose page id is outside 0 .. num_pages - 1 counts as masked (attend) or is not written (append, evict), and both set
+ * bits of *status. Calls allocate nothing, synchronise nothing and may be captured into a HIP graph; lengths and tables
+ * are read when the graph runs. A workspace belongs to one call at a time. The calls leave the thread's current device as
+ * they found it. */
+#define TACO_KV_F32 0
+#define TACO_KV_BF16 1
+#define TACO_KV_F16 2
+#define TACO_KV_BAD_PAGE 1
+#define TACO_KV_BAD_LENGTH 2
+
+typedef struct TacoKvPool {
+    uint32_t struct_size;         /* = sizeof(TacoKvPool) */
+    int32_t device;
+    int32_t dtype;                /* TACO_KV_F32 / BF16 / F16: of the pool, the new rows, the queries and the output */
+    int32_t num_pages;
+    int32_t kv_heads;             /* 1 .. 1024 */
+    int32_t page_size;            /* tokens: 8, 16, 32, 64, 128 or 256 */
+    int32_t head_dim;             /* 64, 128 or 256 */
+    int32_t reserved;             /* 0 */
+    void* k;                      /* [num_pages, kv_heads, page_size, head_dim] by the strides below */
+    void* v;
+    int64_t k_page_stride, k_head_stride, k_token_stride;
+    int64_t v_page_stride, v_head_stride, v_token_stride;
+    int32_t* status;              /* device int32[1], zeroed by the caller: TACO_KV_BAD_* bits are or-ed into it */
+} TacoKvPool;
+
+/* Rows into pages: token t < counts[b] of sequence b goes to slot starts[b] + t, that is row slot % page_size of page
+ * table[b][slot / page_size]; tokens from counts[b] on, and pages of no token, stay untouched.
+ *   table [B, max_pages] int32, rows table_ld apart; starts, counts, first [B] int32 (counts NULL = T each)
+ *   k, v [B, T, kv_heads, head_dim]: strides of batch, token, head
+ *   mass [B, kv_heads, side_ld] fp32, or NULL: 0 for the new slots
+ *   positions [B, kv_heads, side_ld] int32, or NULL: first[b] + t (first NULL = starts) for the new slots
+ *   lengths_out [B] int32: starts[b] + counts[b]
+ * side_ld >= max_pages * page_size. Tokens beyond the table's capacity are dropped (TACO_KV_BAD_LENGTH). The pages that
+ * are written must be the sequence's own. */
+int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
+                   const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                   const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride, int32_t T,
+                   const int32_t* starts, const int32_t* counts, const int32_t* first, float* mass, int32_t* positions,
+                   int64_t side_ld, int32_t* lengths_out, taco_stream_t stream);
+
+/* One new token per sequence: with s[h][t] = scale * q[b][h] . k[b][h / group][t] over slots t < lengths[b],
+ *   lse[b][h] = log sum_t exp s[h][t],   out[b][h] = sum_t exp(s[h][t] - lse[b][h]) v[b][h / group][t],
+ *   mass[b][j][t] += sum over the `group` query heads h of kv head j of exp(s[h][t] - lse[b][h])      (mass not NULL)
+ * q [B, q_heads, head_dim] by strides of batch and head, q_heads = group * kv_heads; out [B, q_heads, head_dim] and
+ * lse [B, q_heads] (fp32, natural log) contiguous; mass [B, kv_heads, side_ld] fp32. Pages may be shared between
+ * sequences. A row without tokens, or whose scores are all -inf, gives out 0 and lse -inf and leaves its mass alone.
+ * What masked slots and unused pages hold (NaN, infinities) has no influence. Sums and softmax statistics are fp32. */
+size_t taco_kv_attend_workspace_bytes(const TacoKvPool* pool, int32_t B, int32_t q_heads, int32_t max_pages,
+                                      int32_t with_mass);
+int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
+                   const int32_t* lengths, const void* q, int64_t q_batch_stride, int64_t q_head_stride, int32_t q_heads,
+                   float scale, void* out, float* lse, float* mass, int64_t side_ld, void* ws, size_t ws_bytes,
+                   taco_stream_t stream);
+
+/* Every (sequence, kv head) is cut to n = min(lengths[b], budget) tokens: the `recent` newest by position (those above
+ * the greatest position - recent), then the greatest masses; of equal masses the lower slot stays, NaN counts as the
+ * greatest. Kept slots below n stay where they are; the empty slots below n take the kept ones from n on, both in
+ * ascending order, so no more rows move than have to (one per head when a sequence is one over its budget) and attention,
+ * which does not depend on the order of slots, goes on. positions says which token a slot holds.
+ *   mass, positions [B, kv_heads, side_ld] -> mass_out, positions_out: slots >= n get 0 and -1
+ *   lengths_out [B]: n.  Each output may be the matching input itself; no other overlap.
+ * Pages of slots >= n may be reused by the caller afterwards. The pages that are written must be the sequence's own.
+ * 0 <= recent <= budget, 1 <= budget. */
+size_t taco_kv_evict_workspace_bytes(const TacoKvPool* pool, int32_t B, int32_t max_pages, int32_t budget);
+int taco_kv_evict(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
+                  const int32_t* lengths, const float* mass, const int32_t* positions, int64_t side_ld, int32_t budget,
+                  int32_t recent, int32_t* lengths_out, float* mass_out, int32_t* positions_out, void* ws,
+                  size_t ws_bytes, taco_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

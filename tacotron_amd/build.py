@@ -11,7 +11,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(HERE, 'csrc', 'build')
 LIB = os.path.join(HERE, 'libtaco_hip.so')
-SOURCES = ['api.hip', 'gemm.hip', 'rnn.hip', 'decoder.hip', 'dec_persistent.hip', 'dec_tile.hip', 'griffinlim.hip']
+SOURCES = ['api.hip', 'gemm.hip', 'rnn.hip', 'decoder.hip', 'dec_persistent.hip', 'dec_tile.hip', 'griffinlim.hip',
+           'kv_cache.hip']
 HEADERS = ['kernels.h', 'fft_core.h', 'dec_common.h', os.path.join('..', '..', 'include', 'taco.h')]
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function']

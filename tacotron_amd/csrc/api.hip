@@ -1631,3 +1631,171 @@ extern "C" int taco_debug_conv_gemm(const float* X, int32_t ldx, int32_t M, int3
     launch_conv_gemm(g, (hipStream_t)stream, nullptr);
     return check_launch("taco_debug_conv_gemm");
 }
+
+// ---------------------------------------------------------------------------------------
+// paged key-value cache
+namespace {
+
+// The call's device for its launches; the thread's current device again afterwards.
+struct DeviceScope {
+    int prev = -1;
+    bool ok = true;
+    explicit DeviceScope(int device) {
+        if (hipGetDevice(&prev) != hipSuccess) { ok = false; prev = -1; return; }
+        if (prev == device) prev = -1;
+        else ok = hipSetDevice(device) == hipSuccess;
+    }
+    ~DeviceScope() { if (prev >= 0) (void)hipSetDevice(prev); }
+};
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int kv_pool_view(const char* what, const TacoKvPool* pool, KvPool* p) {
+    if (!pool) return fail("%s: null pool", what);
+    if (pool->struct_size != sizeof(TacoKvPool))
+        return fail("%s: TacoKvPool.struct_size is %u, this library expects %zu", what, pool->struct_size, sizeof(TacoKvPool));
+    if (!pool->k || !pool->v || !pool->status) return fail("%s: null pool tensor", what);
+    if (pool->dtype < TACO_KV_F32 || pool->dtype > TACO_KV_F16) return fail("%s: dtype %d is not fp32, bf16 or fp16", what, pool->dtype);
+    if (pool->device < 0) return fail("%s: device %d", what, pool->device);
+    if (pool->num_pages < 1) return fail("%s: the pool needs at least one page", what);
+    if (pool->kv_heads < 1 || pool->kv_heads > 1024) return fail("%s: kv_heads must be 1..1024 (got %d)", what, pool->kv_heads);
+    const int ps = pool->page_size, d = pool->head_dim;
+    if (ps < 8 || ps > 256 || (ps & (ps - 1))) return fail("%s: page_size must be 8, 16, 32, 64, 128 or 256 (got %d)", what, ps);
+    if (d != 64 && d != 128 && d != 256) return fail("%s: head_dim must be 64, 128 or 256 (got %d)", what, d);
+    const int esize = pool->dtype == TACO_KV_F32 ? 4 : 2;
+    const int64_t st[6] = {pool->k_page_stride, pool->k_head_stride, pool->k_token_stride,
+                           pool->v_page_stride, pool->v_head_stride, pool->v_token_stride};
+    for (int64_t x : st)
+        if (x < 0 || (x * esize) % 16) return fail("%s: pool strides must be non-negative multiples of 16 bytes", what);
+    if (!aligned16(pool->k) || !aligned16(pool->v)) return fail("%s: the pool must start on a 16-byte boundary", what);
+    p->k = pool->k;
+    p->v = pool->v;
+    for (int i = 0; i < 3; ++i) { p->k_st[i] = st[i]; p->v_st[i] = st[3 + i]; }
+    p->dtype = pool->dtype;
+    p->esize = esize;
+    p->num_pages = pool->num_pages;
+    p->heads = pool->kv_heads;
+    p->page_size = ps;
+    p->page_shift = __builtin_ctz((unsigned)ps);
+    p->dim = d;
+    p->status = pool->status;
+    return 0;
+}
+
+int kv_sizes(const char* what, const KvPool& p, int B, int max_pages) {
+    if (B < 1 || B > 65535) return fail("%s: B must be 1..65535 (got %d)", what, B);
+    if (max_pages < 1 || max_pages > (1 << 30) / p.page_size)
+        return fail("%s: max_pages * page_size must be 1..2^30 (got %d * %d)", what, max_pages, p.page_size);
+    return 0;
+}
+
+int kv_table_view(const char* what, const KvPool& p, const int32_t* table, int64_t ld, int B, int max_pages, KvTable* t) {
+    if (int rc = kv_sizes(what, p, B, max_pages)) return rc;
+    if (!table || ld < max_pages) return fail("%s: null page table, or rows closer than max_pages", what);
+    *t = KvTable{table, ld, B, max_pages};
+    return 0;
+}
+
+int kv_side(const char* what, const KvPool& p, const KvTable& t, int64_t side_ld) {
+    if (side_ld < ((int64_t)t.max_pages << p.page_shift) || side_ld > (1 << 30))
+        return fail("%s: side tables need a row for every slot, max_pages * page_size = %lld, and at most 2^30 (got %lld)",
+                    what, (long long)t.max_pages << p.page_shift, (long long)side_ld);
+    return 0;
+}
+
+int kv_rows(const char* what, const KvPool& p, const void* x, const int64_t* st, int n) {
+    if (!x || !aligned16(x)) return fail("%s: null tensor, or one that does not start on a 16-byte boundary", what);
+    for (int i = 0; i < n; ++i)
+        if (st[i] < 0 || (st[i] * p.esize) % 16) return fail("%s: strides must be non-negative multiples of 16 bytes", what);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
+                              const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                              const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                              int32_t T, const int32_t* starts, const int32_t* counts, const int32_t* first, float* mass,
+                              int32_t* positions, int64_t side_ld, int32_t* lengths_out, taco_stream_t stream) {
+    const char* what = "taco_kv_append";
+    KvPool p;
+    KvTable t;
+    if (int rc = kv_pool_view(what, pool, &p)) return rc;
+    if (int rc = kv_table_view(what, p, table, table_ld, B, max_pages, &t)) return rc;
+    KvAppend a{k, v, {k_batch_stride, k_token_stride, k_head_stride}, {v_batch_stride, v_token_stride, v_head_stride},
+               T, starts, counts, first, mass, positions, side_ld, lengths_out};
+    if (int rc = kv_rows(what, p, k, a.k_st, 3)) return rc;
+    if (int rc = kv_rows(what, p, v, a.v_st, 3)) return rc;
+    if (T < 1 || (int64_t)T * p.heads > (1 << 26)) return fail("%s: T must be at least 1 and T * kv_heads at most 2^26 (got T %d)", what, T);
+    if (!starts || !lengths_out) return fail("%s: null argument", what);
+    if (mass || positions)
+        if (int rc = kv_side(what, p, t, side_ld)) return rc;
+    DeviceScope scope(pool->device);
+    if (!scope.ok) return fail("%s: device %d is not available", what, pool->device);
+    launch_kv_append(p, t, a, (hipStream_t)stream);
+    return check_launch(what);
+}
+
+extern "C" size_t taco_kv_attend_workspace_bytes(const TacoKvPool* pool, int32_t B, int32_t q_heads, int32_t max_pages,
+                                                 int32_t with_mass) {
+    const char* what = "taco_kv_attend_workspace_bytes";
+    KvPool p;
+    if (kv_pool_view(what, pool, &p) || kv_sizes(what, p, B, max_pages)) return 0;
+    if (q_heads < 1 || q_heads % p.heads) { (void)fail("%s: q_heads must be a multiple of kv_heads", what); return 0; }
+    return std::max<size_t>(kv_attend_ws_bytes(p, B, q_heads / p.heads, max_pages, with_mass != 0), 16);
+}
+
+extern "C" int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B,
+                              int32_t max_pages, const int32_t* lengths, const void* q, int64_t q_batch_stride,
+                              int64_t q_head_stride, int32_t q_heads, float scale, void* out, float* lse, float* mass,
+                              int64_t side_ld, void* ws, size_t ws_bytes, taco_stream_t stream) {
+    const char* what = "taco_kv_attend";
+    KvPool p;
+    KvTable t;
+    if (int rc = kv_pool_view(what, pool, &p)) return rc;
+    if (int rc = kv_table_view(what, p, table, table_ld, B, max_pages, &t)) return rc;
+    if (q_heads < 1 || q_heads > 65535 || q_heads % p.heads)
+        return fail("%s: q_heads must be a multiple of kv_heads, at most 65535 (got %d over %d)", what, q_heads, p.heads);
+    KvAttend a{q, {q_batch_stride, q_head_stride}, q_heads / p.heads, lengths, scale * 1.4426950408889634f, out, lse, mass, side_ld};
+    if (int rc = kv_rows(what, p, q, a.q_st, 2)) return rc;
+    if (!lengths || !out || !lse || !aligned16(out)) return fail("%s: null argument, or out not on a 16-byte boundary", what);
+    if (!std::isfinite(scale)) return fail("%s: scale must be finite", what);
+    if (mass)
+        if (int rc = kv_side(what, p, t, side_ld)) return rc;
+    if (!ws || !aligned16(ws) || ws_bytes < kv_attend_ws_bytes(p, B, a.group, max_pages, mass != nullptr))
+        return fail("%s: workspace too small (taco_kv_attend_workspace_bytes) or not on a 16-byte boundary", what);
+    DeviceScope scope(pool->device);
+    if (!scope.ok) return fail("%s: device %d is not available", what, pool->device);
+    launch_kv_attend(p, t, a, (hipStream_t)stream);
+    return check_launch(what);
+}
+
+extern "C" size_t taco_kv_evict_workspace_bytes(const TacoKvPool* pool, int32_t B, int32_t max_pages, int32_t budget) {
+    const char* what = "taco_kv_evict_workspace_bytes";
+    KvPool p;
+    if (kv_pool_view(what, pool, &p) || kv_sizes(what, p, B, max_pages)) return 0;
+    if (budget < 1) { (void)fail("%s: budget must be at least 1", what); return 0; }
+    return kv_evict_ws_bytes(p, B, max_pages, budget);
+}
+
+extern "C" int taco_kv_evict(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
+                             const int32_t* lengths, const float* mass, const int32_t* positions, int64_t side_ld,
+                             int32_t budget, int32_t recent, int32_t* lengths_out, float* mass_out,
+                             int32_t* positions_out, void* ws, size_t ws_bytes, taco_stream_t stream) {
+    const char* what = "taco_kv_evict";
+    KvPool p;
+    KvTable t;
+    if (int rc = kv_pool_view(what, pool, &p)) return rc;
+    if (int rc = kv_table_view(what, p, table, table_ld, B, max_pages, &t)) return rc;
+    if (!lengths || !mass || !positions || !lengths_out || !mass_out || !positions_out) return fail("%s: null argument", what);
+    if (int rc = kv_side(what, p, t, side_ld)) return rc;
+    if (budget < 1 || recent < 0 || recent > budget)
+        return fail("%s: needs 0 <= recent <= budget and budget >= 1 (got recent %d, budget %d)", what, recent, budget);
+    if (!ws || !aligned16(ws) || ws_bytes < kv_evict_ws_bytes(p, B, max_pages, budget))
+        return fail("%s: workspace too small (taco_kv_evict_workspace_bytes) or not on a 16-byte boundary", what);
+    DeviceScope scope(pool->device);
+    if (!scope.ok) return fail("%s: device %d is not available", what, pool->device);
+    KvEvict a{lengths, budget, recent, mass, positions, side_ld, lengths_out, mass_out, positions_out, nullptr, nullptr, 0};
+    launch_kv_evict(p, t, a, ws, (hipStream_t)stream);
+    return check_launch(what);
+}

@@ -246,4 +246,44 @@ void launch_gl_ola_norm(const GLPlan& p, const float* frames, float* wav, int B,
 void launch_stft_center(const GLPlan& p, const float* wav, int B, int n, int T, float preemph, float ref_db,
                         float min_db, float* mag, int ldm, float* lin, hipStream_t s, Timing* tm);
 
+// ---------------------------------------------------------------------------------------
+// Paged key-value cache (kv_cache.hip; include/taco.h: taco_kv_*). Host-checked views of the caller's arguments.
+enum KvType : int { KV_F32 = 0, KV_BF16 = 1, KV_F16 = 2 };
+enum KvStatus : int { KV_BAD_PAGE = 1, KV_BAD_LENGTH = 2 };
+struct KvPool {
+    void* k; void* v;                     // [num_pages] x [heads] x [page_size] rows of dim elements
+    int64_t k_st[3], v_st[3];             // strides in elements: page, head, token
+    int dtype, esize;
+    int num_pages, heads, page_size, page_shift, dim;
+    int32_t* status;
+};
+struct KvTable { const int32_t* table; int64_t ld; int B, max_pages; };
+struct KvAppend {
+    const void* k; const void* v;         // [B] x [T] x [heads] rows
+    int64_t k_st[3], v_st[3];             // batch, token, head
+    int T;
+    const int32_t* starts; const int32_t* counts; const int32_t* first;
+    float* mass; int32_t* positions; int64_t side_ld;
+    int32_t* lengths_out;
+};
+struct KvAttend {
+    const void* q; int64_t q_st[2];       // [B] x [heads * group] rows: batch, head
+    int group;
+    const int32_t* lengths;
+    float scale2;                         // scale * log2(e): scores are kept in units of ln 2
+    void* out; float* lse;                // contiguous
+    float* mass; int64_t side_ld;
+};
+struct KvEvict {
+    const int32_t* lengths; int budget, recent;
+    const float* mass; const int32_t* positions; int64_t side_ld;
+    int32_t* lengths_out; float* mass_out; int32_t* positions_out;
+    int32_t* counts; int32_t* lists; int64_t list_ld;      // workspace
+};
+void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hipStream_t s);
+size_t kv_attend_ws_bytes(const KvPool& p, int B, int group, int max_pages, bool mass);
+void launch_kv_attend(const KvPool& p, const KvTable& tb, const KvAttend& a, hipStream_t s);
+size_t kv_evict_ws_bytes(const KvPool& p, int B, int max_pages, int budget);
+void launch_kv_evict(const KvPool& p, const KvTable& tb, KvEvict a, void* ws, hipStream_t s);
+
 }  // namespace taco
