@@ -1671,6 +1671,7 @@ int kv_pool_view(const char* what, const TacoKvPool* pool, KvPool* p) {
     p->k = pool->k;
     p->v = pool->v;
     for (int i = 0; i < 3; ++i) { p->k_st[i] = st[i]; p->v_st[i] = st[3 + i]; }
+    p->device = pool->device;
     p->dtype = pool->dtype;
     p->esize = esize;
     p->num_pages = pool->num_pages;
@@ -1700,6 +1701,14 @@ int kv_side(const char* what, const KvPool& p, const KvTable& t, int64_t side_ld
     if (side_ld < ((int64_t)t.max_pages << p.page_shift) || side_ld > (1 << 30))
         return fail("%s: side tables need a row for every slot, max_pages * page_size = %lld, and at most 2^30 (got %lld)",
                     what, (long long)t.max_pages << p.page_shift, (long long)side_ld);
+    return 0;
+}
+
+int kv_heads_ok(const char* what, const KvPool& p, int B, int q_heads, int max_pages) {
+    if (q_heads < 1 || q_heads > 65535 || q_heads % p.heads)
+        return fail("%s: q_heads must be a multiple of kv_heads, at most 65535 (got %d over %d)", what, q_heads, p.heads);
+    if (!kv_attend_fits(p, B, q_heads / p.heads, max_pages))
+        return fail("%s: B * q_heads and B * kv_heads * slots are too many for one call", what);
     return 0;
 }
 
@@ -1741,7 +1750,7 @@ extern "C" size_t taco_kv_attend_workspace_bytes(const TacoKvPool* pool, int32_t
     const char* what = "taco_kv_attend_workspace_bytes";
     KvPool p;
     if (kv_pool_view(what, pool, &p) || kv_sizes(what, p, B, max_pages)) return 0;
-    if (q_heads < 1 || q_heads % p.heads) { (void)fail("%s: q_heads must be a multiple of kv_heads", what); return 0; }
+    if (kv_heads_ok(what, p, B, q_heads, max_pages)) return 0;
     return std::max<size_t>(kv_attend_ws_bytes(p, B, q_heads / p.heads, max_pages, with_mass != 0), 16);
 }
 
@@ -1754,9 +1763,9 @@ extern "C" int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int6
     KvTable t;
     if (int rc = kv_pool_view(what, pool, &p)) return rc;
     if (int rc = kv_table_view(what, p, table, table_ld, B, max_pages, &t)) return rc;
-    if (q_heads < 1 || q_heads > 65535 || q_heads % p.heads)
-        return fail("%s: q_heads must be a multiple of kv_heads, at most 65535 (got %d over %d)", what, q_heads, p.heads);
-    KvAttend a{q, {q_batch_stride, q_head_stride}, q_heads / p.heads, lengths, scale * 1.4426950408889634f, out, lse, mass, side_ld};
+    if (int rc = kv_heads_ok(what, p, B, q_heads, max_pages)) return rc;
+    KvAttend a{q, {q_batch_stride, q_head_stride}, q_heads / p.heads, lengths, scale * 1.4426950408889634f, out, lse, mass, side_ld,
+               nullptr, nullptr, nullptr, 0};
     if (int rc = kv_rows(what, p, q, a.q_st, 2)) return rc;
     if (!lengths || !out || !lse || !aligned16(out)) return fail("%s: null argument, or out not on a 16-byte boundary", what);
     if (!std::isfinite(scale)) return fail("%s: scale must be finite", what);
@@ -1766,7 +1775,7 @@ extern "C" int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int6
         return fail("%s: workspace too small (taco_kv_attend_workspace_bytes) or not on a 16-byte boundary", what);
     DeviceScope scope(pool->device);
     if (!scope.ok) return fail("%s: device %d is not available", what, pool->device);
-    launch_kv_attend(p, t, a, (hipStream_t)stream);
+    launch_kv_attend(p, t, a, ws, (hipStream_t)stream);
     return check_launch(what);
 }
 

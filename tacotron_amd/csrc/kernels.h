@@ -253,7 +253,7 @@ enum KvStatus : int { KV_BAD_PAGE = 1, KV_BAD_LENGTH = 2 };
 struct KvPool {
     void* k; void* v;                     // [num_pages] x [heads] x [page_size] rows of dim elements
     int64_t k_st[3], v_st[3];             // strides in elements: page, head, token
-    int dtype, esize;
+    int device, dtype, esize;
     int num_pages, heads, page_size, page_shift, dim;
     int32_t* status;
 };
@@ -273,6 +273,9 @@ struct KvAttend {
     float scale2;                         // scale * log2(e): scores are kept in units of ln 2
     void* out; float* lse;                // contiguous
     float* mass; int64_t side_ld;
+    // workspace: parts of heads that several workgroups share, [2 * workgroups][16] {maximum, sum} and
+    // [2 * workgroups][score_rows][dim]; with mass, the scores, [units][score_rows][unit]
+    float2* part_ml; float* part_out; float* scores; int score_rows;
 };
 struct KvEvict {
     const int32_t* lengths; int budget, recent;
@@ -281,8 +284,9 @@ struct KvEvict {
     int32_t* counts; int32_t* lists; int64_t list_ld;      // workspace
 };
 void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hipStream_t s);
+bool kv_attend_fits(const KvPool& p, int B, int group, int max_pages);
 size_t kv_attend_ws_bytes(const KvPool& p, int B, int group, int max_pages, bool mass);
-void launch_kv_attend(const KvPool& p, const KvTable& tb, const KvAttend& a, hipStream_t s);
+void launch_kv_attend(const KvPool& p, const KvTable& tb, KvAttend a, void* ws, hipStream_t s);
 size_t kv_evict_ws_bytes(const KvPool& p, int B, int max_pages, int budget);
 void launch_kv_evict(const KvPool& p, const KvTable& tb, KvEvict a, void* ws, hipStream_t s);
 

@@ -8,6 +8,9 @@
 // status word. Offsets into the pool and the side tables are 64-bit.
 #include "kernels.h"
 
+#include <atomic>
+#include <type_traits>
+
 namespace taco {
 namespace {
 
@@ -75,83 +78,488 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvPool p, const Kv
 
 // ---------------------------------------------------------------------------------------
 // attend
+//
+// One pass over the pages with the running maximum and sum of the softmax, on the matrix cores, the token axis cut into
+// equal shares. What bounds it is reading K and V once.
+//
+// Shares. The tokens of a (sequence, kv head) are units of 4 waves x TW tokens; all units of the call, sequence by
+// sequence and head by head, are one line, and workgroup w of W takes the w-th W-th of it. The line is laid out on the
+// device from the lengths, so the split follows the lengths that are there when the kernel (or a captured graph) runs, a
+// ragged batch is as balanced as an even one, and one long sequence fills the chip. Where a head's units end up in several
+// workgroups each leaves {maximum, sum, unnormalised output} in the workspace and kv_join_kernel joins them.
+//
+// Products. Query heads of one kv head are the columns of 16-wide tiles (a group over 16 takes several passes, one under
+// 16 leaves columns idle: the matrix cores have the room, the reads of K and V are what counts).
+//   S^T = K Q^T: a lane of the A operand is a token (lane & 15) with 16 bytes of its row at 16 (lane >> 4) + 64 j; the
+//     order of the summed dimension is free as long as Q has the same, so both are plain 16-byte loads.
+//   O^T += V^T P^T: the C layout of S^T leaves lane (g = lane >> 4, head = lane & 15) with tokens 4 g + i of every 16, which
+//     is the B operand as it stands when the summed tokens are taken in that order. A lane loads VEC consecutive
+//     dims of each of those tokens, 16 lanes a whole row; for 16-bit types the 8 x VEC block it holds is
+//     transposed in registers (one v_perm per dword). No LDS, no barrier in the loop.
+// fp32 runs on v_mfma_f32_16x16x4_f32, 16-bit types on the 16x16x32 ones.
 
-template <typename T>
-__device__ __forceinline__ float dot_row(const T* q, const T* k, int dim) {
-    float s = 0.f;
-    for (int d = 0; d < dim; ++d) s += (float)q[d] * (float)k[d];
-    return s;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int AT_WAVES = 4;
+constexpr int AT_JOIN_MAX = 2048;        // workgroups, at most: parts of a head that kv_join_kernel has room for
+constexpr int MASS_TOKENS = 1024;        // tokens of mass per workgroup
+
+template <int DT, int D>
+struct AttendShape {
+    static constexpr int ES = DT == KV_F32 ? 4 : 2;
+    static constexpr int TW = DT == KV_F32 ? 16 : 32;          // tokens of a wave's tile
+    static constexpr int UNIT = AT_WAVES * TW;
+    static constexpr int VEC = DT != KV_F32 && D >= 128 ? 8 : 4;   // dims per lane and V row
+    static constexpr int NX = D / (16 * VEC);
+    static constexpr int NACC = D / 16;
+    static constexpr int KL = D * ES / 64;                     // 16-byte loads per lane and K row
+};
+
+int attend_unit(int dtype) { return dtype == KV_F32 ? AttendShape<KV_F32, 64>::UNIT : AttendShape<KV_BF16, 64>::UNIT; }
+
+__device__ __forceinline__ int wave_sum(int x) {
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    return x;
 }
 
-// Score (in units of ln 2) of query row q against slot t, or -inf where its page id is bad.
-template <typename T>
-__device__ __forceinline__ float slot_score(const KvPool& p, const int32_t* row, const T* q, int h, int t, float scale2,
-                                            bool report) {
-    const int page = row[t >> p.page_shift];
-    if ((unsigned)page >= (unsigned)p.num_pages) {
-        if (report) atomicOr(p.status, KV_BAD_PAGE);
-        return -INFINITY;
+// The line of units: sequence b has units(len_b) of them for each of H head groups.
+struct Line {
+    int base, rem;                       // share w: base units, and one more for w < rem
+    __device__ Line(int U, int W) : base(U / W), rem(U % W) {}
+    __device__ int begin(int w) const { return w * base + min(w, rem); }
+    __device__ int share_of(int u) const {
+        const int big = rem * (base + 1);
+        return u < big ? u / (base + 1) : rem + (u - big) / base;
     }
-    return dot_row(q, (const T*)p.k + slot_off(p.k_st, page, h, t & (p.page_size - 1)), p.dim) * scale2;
+};
+
+__device__ __forceinline__ int units_of(const KvTable& tb, const int32_t* lengths, int b, int cap, int unit) {
+    const int n = lengths[b];
+    return n <= 0 ? 0 : (min(n, cap) + unit - 1) / unit;
 }
 
-// One workgroup per (sequence, query head): 256 tokens at a time, a score per thread, the running maximum and sum of the
-// softmax, then a column of the output per thread.
-template <typename T>
+template <int DT>
+struct Mma;
+template <>
+struct Mma<KV_BF16> {
+    static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<KV_F16> {
+    static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<KV_F32> {
+    static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+        return c;
+    }
+};
+
+// Two 16-bit halves of a weight: hi + lo holds it to 2^-16 (bf16) or 2^-21 (fp16), so that the second product loses nothing
+// against 32-bit weights. One more matrix instruction per tile; the kernel waits for memory either way.
+template <typename V8>
+__device__ __forceinline__ void split8(const float* p, u32x4* hi, u32x4* lo) {
+    V8 h, l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        h[i] = (decltype(h[0] + h[0]))p[i];
+        l[i] = (decltype(h[0] + h[0]))(p[i] - (float)h[i]);
+    }
+    *hi = __builtin_bit_cast(u32x4, h);
+    *lo = __builtin_bit_cast(u32x4, l);
+}
+
+template <int DT, int D, bool MASS>
 __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
-    __shared__ float w[256], red[256];
-    const int hq = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const int h = hq / a.group, cap = tb.max_pages << p.page_shift;
-    const int len = clamp_len(a.lengths[b], cap, p.status, hq == 0 && tid == 0);
-    const int32_t* row = tb.table + (int64_t)b * tb.ld;
-    const T* q = (const T*)a.q + (int64_t)b * a.q_st[0] + (int64_t)hq * a.q_st[1];
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    for (int t0 = 0; t0 < len; t0 += 256) {
-        const int t = t0 + tid, n = min(256, len - t0);
-        const float s = t < len ? slot_score(p, row, q, h, t, a.scale2, true) : -INFINITY;
-        red[tid] = s;
-        __syncthreads();
-        float mx = m;
-        for (int i = 0; i < n; ++i) mx = fmaxf(mx, red[i]);
-        const float mr = mx == -INFINITY ? 0.f : mx;
-        const float alpha = ex2(m - mr);
-        w[tid] = ex2(s - mr);
-        __syncthreads();
-        // the chunk's sums first: thousands of small equal weights added to a large total one by one would all round
-        // the same way
-        float lc = 0.f, accc = 0.f;
-        for (int i = 0; i < n; ++i) {
-            lc += w[i];
-            const int page = row[(t0 + i) >> p.page_shift];
-            if (tid < p.dim && (unsigned)page < (unsigned)p.num_pages)
-                accc += w[i] * (float)((const T*)p.v + slot_off(p.v_st, page, h, (t0 + i) & (p.page_size - 1)))[tid];
+    using S = AttendShape<DT, D>;
+    constexpr int TW = S::TW, UNIT = S::UNIT, VEC = S::VEC, NX = S::NX, NACC = S::NACC, KL = S::KL, ES = S::ES;
+    constexpr int NS = TW / 16, NV = TW / 4;         // 16-token blocks; tokens a lane holds
+    // fp16 weights are kept 2^14 too large (the sums with them): at most 16384, and 2^-28 is still a normal number, so that
+    // many small weights beside a large one are not lost
+    constexpr float OFF = DT == KV_F16 ? 14.f : 0.f;
+    typedef typename std::conditional<VEC * ES == 16, u32x4, u32x2>::type vload_t;
+    __shared__ float xch[4][3][NACC][64];            // quarter, source wave, accumulator, lane
+    __shared__ float2 ml[AT_WAVES][16];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int cap = tb.max_pages << p.page_shift, w = blockIdx.x, W = gridDim.x;
+    const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
+
+    // sequences without tokens, and the check of the lengths
+    for (int b = w; b < tb.B; b += W)
+        if (clamp_len(a.lengths[b], cap, p.status, tid == 0) == 0) {
+            for (int i = tid; i < hq * D * ES / 4; i += 256) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
+            for (int i = tid; i < hq; i += 256) a.lse[(int64_t)b * hq + i] = -INFINITY;
         }
-        l = l * alpha + lc;
-        acc = acc * alpha + accc;
-        m = mx;
-        __syncthreads();
+
+    int total = 0;
+    for (int i = lane; i < tb.B; i += 64) total += units_of(tb, a.lengths, i, cap, UNIT);
+    total = __builtin_amdgcn_readfirstlane(wave_sum(total));
+    const Line line(total * H, W);
+    const int u0 = line.begin(w), u1 = line.begin(w + 1);
+    if (u0 == u1) return;
+    int b = 0, before = 0;                           // the sequence of unit u0, and the units before it
+    for (int b0 = 0;; b0 += 64) {
+        const int x = b0 + lane < tb.B ? units_of(tb, a.lengths, b0 + lane, cap, UNIT) * H : 0;
+        int inc = x;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(inc, o);
+            if (lane >= o) inc += y;
+        }
+        const unsigned long long hit = __ballot(before + inc > u0);
+        if (hit) {
+            const int at = __ffsll(hit) - 1;
+            b = b0 + at;
+            before += __shfl(inc - x, at);
+            break;
+        }
+        before += __shfl(inc, 63);
     }
-    // a row that saw no token, or none with a score above -inf: 0 and -inf
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (tid < p.dim) ((T*)a.out)[((int64_t)b * gridDim.x + hq) * p.dim + tid] = (T)(acc * inv);
-    if (tid == 0) a.lse[(int64_t)b * gridDim.x + hq] = l == 0.f ? -INFINITY : m * LN2 + logf(l);
+    b = __builtin_amdgcn_readfirstlane(b);
+    before = __builtin_amdgcn_readfirstlane(before);
+    int nb = units_of(tb, a.lengths, b, cap, UNIT);
+    int hg = (u0 - before) / nb, tile = (u0 - before) % nb;
+
+    for (int u = u0; u < u1;) {
+        const int stop = min(nb, tile + (u1 - u));
+        const int len = min(a.lengths[b], cap);
+        const int kvh = hg / ngrp, head0 = kvh * a.group + (hg % ngrp) * 16, nh = min(16, a.group - (hg % ngrp) * 16);
+        const int tend = min(len, stop * UNIT);
+        const int32_t* row = tb.table + (int64_t)b * tb.ld;
+        const char* kbase = (const char*)p.k + (int64_t)kvh * p.k_st[1] * ES;
+        const char* vbase = (const char*)p.v + (int64_t)kvh * p.v_st[1] * ES;
+        const int64_t kp = p.k_st[0] * ES, kt = p.k_st[2] * ES, vp = p.v_st[0] * ES, vt = p.v_st[2] * ES;
+        const int mask = p.page_size - 1;
+
+        u32x4 qf[KL];
+        const char* q = (const char*)a.q + ((int64_t)b * a.q_st[0] + (int64_t)(head0 + col) * a.q_st[1]) * ES + grp * 16;
+#pragma unroll
+        for (int j = 0; j < KL; ++j) qf[j] = col < nh ? *reinterpret_cast<const u32x4*>(q + j * 64) : u32x4{0, 0, 0, 0};
+
+        float m = -INFINITY, l = 0.f;
+        f32x4 acc[NACC];
+#pragma unroll
+        for (int n = 0; n < NACC; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        // page of slot t (t may lie behind the share: the last slot's then, masked later)
+        auto page_of = [&](int t) { return row[min(t, tend - 1) >> p.page_shift]; };
+        auto good = [&](int t, int page) { return t < tend && (unsigned)page < (unsigned)p.num_pages; };
+        u32x4 kf[NS][KL];
+        auto load_k = [&](int t, const int* page) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const int tok = t + 16 * s + col;
+                // a masked slot reads the pool's first row: its score is replaced
+                const char* r = good(tok, page[s]) ? kbase + page[s] * kp + (tok & mask) * kt : (const char*)p.k;
+#pragma unroll
+                for (int j = 0; j < KL; ++j) kf[s][j] = *reinterpret_cast<const u32x4*>(r + grp * 16 + j * 64);
+            }
+        };
+        int t = tile * UNIT + wave * TW;
+        int kpage[NS], vpage[NS];
+        if (t < tend) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) { kpage[s] = page_of(t + 16 * s + col); vpage[s] = page_of(t + 16 * s + 4 * grp); }
+            load_k(t, kpage);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) kpage[s] = page_of(t + UNIT + 16 * s + col);
+        }
+        float* scores = nullptr;
+        if (MASS) scores = a.scores + ((int64_t)(u - tile) * a.score_rows + col) * UNIT + 4 * grp;
+        for (; t < tend; t += UNIT) {
+            // pages of the tile after the next, then V of this one: in flight during the first product
+            int kpage2[NS], vpage2[NS];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                kpage2[s] = page_of(t + 2 * UNIT + 16 * s + col);
+                vpage2[s] = page_of(t + UNIT + 16 * s + 4 * grp);
+            }
+            vload_t vf[NV][NX];
+            bool ok[NS];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const int tok = t + 16 * s + 4 * grp;
+                ok[s] = (unsigned)vpage[s] < (unsigned)p.num_pages;
+                if (!ok[s] && tok < tend) atomicOr(p.status, KV_BAD_PAGE);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const char* r = ok[s] && tok + i < tend ? vbase + vpage[s] * vp + ((tok + i) & mask) * vt : (const char*)p.v;
+#pragma unroll
+                    for (int x = 0; x < NX; ++x) vf[4 * s + i][x] = *reinterpret_cast<const vload_t*>(r + (col + 16 * x) * VEC * ES);
+                }
+            }
+            float sc[NV];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < KL; ++j) c = Mma<DT>::run(kf[s][j], qf[j], c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[4 * s + i] = c[i] * a.scale2;
+            }
+            if (t + UNIT < tend) load_k(t + UNIT, kpage);
+            bool all_ok = t + TW <= tend;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) all_ok &= ok[s];
+            if (!__all(all_ok)) {
+                // masked slots: score -inf, and no row that 0 could be multiplied with to give NaN
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (!(ok[i >> 2] && t + 16 * (i >> 2) + 4 * grp + (i & 3) < tend)) {
+                        sc[i] = -INFINITY;
+#pragma unroll
+                        for (int x = 0; x < NX; ++x) vf[i][x] = vload_t{};
+                    }
+            }
+            if (MASS && col < nh) {
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+                    *reinterpret_cast<f32x4*>(scores + (int64_t)(t / UNIT) * a.score_rows * UNIT + wave * TW + 16 * s) =
+                        f32x4{sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]};
+            }
+            float mx = sc[0];
+#pragma unroll
+            for (int i = 1; i < NV; ++i) mx = fmaxf(mx, sc[i]);
+            if (__any(mx > m)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16));
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const float mn = fmaxf(m, mx);
+                const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+                m = mn;
+                l *= alpha;
+#pragma unroll
+                for (int n = 0; n < NACC; ++n) acc[n] *= alpha;
+            }
+            const float ref = m == -INFINITY ? 0.f : m - OFF;
+            float pr[NV], sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) { pr[i] = ex2(sc[i] - ref); sum += pr[i]; }
+            l += sum;
+            if constexpr (DT == KV_F32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int x = 0; x < NX; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[4 * x + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][x][e]), pr[i], acc[4 * x + e], 0, 0, 0);
+            } else {
+                u32x4 hi, lo;
+                if constexpr (DT == KV_BF16) split8<bf16x8>(pr, &hi, &lo);
+                else split8<f16x8>(pr, &hi, &lo);
+#pragma unroll
+                for (int x = 0; x < NX; ++x)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        u32x4 v;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            v[i] = __builtin_amdgcn_perm(vf[2 * i + 1][x][e >> 1], vf[2 * i][x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                        acc[x * VEC + e] = Mma<DT>::run(v, hi, acc[x * VEC + e]);
+                        acc[x * VEC + e] = Mma<DT>::run(v, lo, acc[x * VEC + e]);
+                    }
+            }
+#pragma unroll
+            for (int s = 0; s < NS; ++s) { kpage[s] = kpage2[s]; vpage[s] = vpage2[s]; }
+        }
+
+        // the four waves' parts: wave r adds up component r of every accumulator, dims x 16 VEC + (4 grp + r) VEC + e
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (grp == 0) ml[wave][col] = float2{m == -INFINITY ? -INFINITY : m - OFF, l};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r != wave) {
+#pragma unroll
+                for (int n = 0; n < NACC; ++n) xch[r][wave - (wave > r)][n][lane] = acc[n][r];
+            }
+        __syncthreads();
+        float M = -INFINITY, L = 0.f, fac[AT_WAVES];
+#pragma unroll
+        for (int i = 0; i < AT_WAVES; ++i) M = fmaxf(M, ml[i][col].x);
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int i = 0; i < AT_WAVES; ++i) { fac[i] = ex2(ml[i][col].x - ref); L += fac[i] * ml[i][col].y; }
+        float o[NACC];
+#pragma unroll
+        for (int n = 0; n < NACC; ++n) {
+            o[n] = (wave == 0 ? acc[n][0] : wave == 1 ? acc[n][1] : wave == 2 ? acc[n][2] : acc[n][3]) * fac[wave];
+#pragma unroll
+            for (int i = 0; i < AT_WAVES; ++i)
+                if (i != wave) o[n] += xch[wave][i - (i > wave)][n][lane] * fac[i];
+        }
+        if (col < nh) {
+            const int d0 = (4 * grp + wave) * VEC;
+            const bool whole = tile == 0 && stop == nb;
+            if (whole) {
+                // no weight at all (every page bad, or every score -inf): as a row without tokens
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                const int64_t head = (int64_t)b * hq + head0 + col;
+                if (wave == 0 && grp == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
+#pragma unroll
+                for (int x = 0; x < NX; ++x)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int64_t at = head * D + x * 16 * VEC + d0 + e;
+                        if constexpr (DT == KV_F32) ((float*)a.out)[at] = o[x * VEC + e] * inv;
+                        else if constexpr (DT == KV_BF16) ((bf16_t*)a.out)[at] = (bf16_t)(o[x * VEC + e] * inv);
+                        else ((f16_t*)a.out)[at] = (f16_t)(o[x * VEC + e] * inv);
+                    }
+            } else {
+                const int slot = 2 * w + (u != u0);
+                if (wave == 0 && grp == 0) a.part_ml[slot * 16 + col] = float2{M, L};
+                float* po = a.part_out + ((int64_t)slot * a.score_rows + col) * D + d0;
+#pragma unroll
+                for (int x = 0; x < NX; ++x)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) po[x * 16 * VEC + e] = o[x * VEC + e];
+            }
+        }
+        u += stop - tile;
+        tile = 0;
+        if (u < u1) {
+            __syncthreads();                         // the exchange is read before the next part writes it
+            if (++hg == H) {
+                hg = 0;
+                do nb = units_of(tb, a.lengths, ++b, cap, UNIT);
+                while (nb == 0);
+            }
+        }
+    }
 }
 
-// mass[b][h][t] += sum over the query heads of kv head h of exp(score - lse): a token per thread.
-template <typename T>
-__global__ __launch_bounds__(256) void kv_mass_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
-    const int h = blockIdx.y, b = blockIdx.z, t = blockIdx.x * 256 + threadIdx.x;
+// Parts of one (sequence, head group): workgroups w0 .. w1, and where part w of them lies in the workspace.
+struct Parts {
+    int first, w0, w1;                   // first unit
+    __device__ int slot(const Line& line, int w) const { return 2 * w + (line.begin(w) < first); }
+};
+
+// Workgroups 0 .. B * hq - 1: the parts of one (sequence, query head) joined. The rest: MASS_TOKENS tokens of
+// mass[b][h] += sum over the query heads of h of exp(score - lse), from the scores that kv_attend_kernel left. The lse of
+// a head in parts is computed by whoever needs it (a few values), so that both fit one launch.
+template <int D>
+__global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTable tb, const KvAttend a, int W, int unit) {
+    __shared__ float fac[AT_JOIN_MAX];
+    __shared__ float sums[256];
+    __shared__ float lse2[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cap = tb.max_pages << p.page_shift;
-    if (t >= clamp_len(a.lengths[b], cap, p.status, false)) return;
-    const int32_t* row = tb.table + (int64_t)b * tb.ld;
-    const int hq = p.heads * a.group;
-    float sum = 0.f;
-    for (int g = 0; g < a.group; ++g) {
-        const T* q = (const T*)a.q + (int64_t)b * a.q_st[0] + (int64_t)(h * a.group + g) * a.q_st[1];
-        const float lse = a.lse[(int64_t)b * hq + h * a.group + g];
-        if (lse != -INFINITY) sum += ex2(slot_score(p, row, q, h, t, a.scale2, false) - lse * LOG2E);
+    const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
+    const int joins = tb.B * hq;
+    const bool join = (int)blockIdx.x < joins;
+    int b, kvh, h0 = 0, t0 = 0;                      // h0: query head within the group
+    if (join) {
+        b = blockIdx.x / hq;
+        kvh = blockIdx.x % hq / a.group;
+        h0 = blockIdx.x % hq % a.group;
+    } else {
+        const int chunks = (cap + MASS_TOKENS - 1) / MASS_TOKENS, i = blockIdx.x - joins;
+        b = i / (chunks * p.heads);
+        kvh = i / chunks % p.heads;
+        t0 = i % chunks * MASS_TOKENS;
     }
-    a.mass[((int64_t)b * p.heads + h) * a.side_ld + t] += sum;
+    const int len = max(0, min(a.lengths[b], cap));
+    if (t0 >= len) return;
+    const int nb = (len + unit - 1) / unit;
+    if (join && nb == 1) return;                     // a single unit is never in parts
+    int total = 0, before = 0;
+    for (int i = lane; i < tb.B; i += 64) {
+        const int n = units_of(tb, a.lengths, i, cap, unit);
+        total += n;
+        before += i < b ? n : 0;
+    }
+    total = __builtin_amdgcn_readfirstlane(wave_sum(total));
+    before = __builtin_amdgcn_readfirstlane(wave_sum(before));
+    const Line line(total * H, W);
+    auto parts_of = [&](int grp16) {
+        Parts q;
+        q.first = before * H + (kvh * ngrp + grp16) * nb;
+        q.w0 = line.share_of(q.first);
+        q.w1 = line.share_of(q.first + nb - 1);
+        return q;
+    };
+    // reference exponent and sum of head c of a group, over its parts: a wave's lanes take a part each
+    auto stats = [&](const Parts& q, int c, float* L) {
+        float M = -INFINITY, sum = 0.f;
+        for (int w = q.w0 + lane; w <= q.w1; w += 64) M = fmaxf(M, a.part_ml[q.slot(line, w) * 16 + c].x);
+        for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+        const float ref = M == -INFINITY ? 0.f : M;
+        for (int w = q.w0 + lane; w <= q.w1; w += 64) {
+            const float2 x = a.part_ml[q.slot(line, w) * 16 + c];
+            sum += x.y * ex2(x.x - ref);
+        }
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        *L = sum;
+        return ref;
+    };
+    if (join) {
+        const Parts q = parts_of(h0 >> 4);
+        if (q.w0 == q.w1) return;
+        const int c = h0 & 15, n = q.w1 - q.w0 + 1;
+        float L;
+        const float ref = stats(q, c, &L);
+        for (int i = tid; i < n; i += 256) fac[i] = ex2(a.part_ml[q.slot(line, q.w0 + i) * 16 + c].x - ref);
+        __syncthreads();
+        const int d = tid % D, k = tid / D;
+        float o = 0.f;
+        for (int i = k; i < n; i += 256 / D) o += fac[i] * a.part_out[((int64_t)q.slot(line, q.w0 + i) * a.score_rows + c) * D + d];
+        sums[tid] = o;
+        __syncthreads();
+        if (tid >= D) return;
+        for (int i = 1; i < 256 / D; ++i) o += sums[tid + i * D];
+        o *= L == 0.f ? 0.f : 1.f / L;
+        const int64_t head = (int64_t)b * hq + kvh * a.group + h0;
+        if (tid == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
+        if (p.dtype == KV_F32) ((float*)a.out)[head * D + d] = o;
+        else if (p.dtype == KV_BF16) ((bf16_t*)a.out)[head * D + d] = (bf16_t)o;
+        else ((f16_t*)a.out)[head * D + d] = (f16_t)o;
+        return;
+    }
+    constexpr int PER = MASS_TOKENS / 256;
+    float sum[PER] = {};
+    for (int g = 0; g < ngrp; ++g) {
+        const Parts q = parts_of(g);
+        const int nh = min(16, a.group - 16 * g);
+        for (int c = wave; c < nh; c += 4) {
+            float x;
+            if (q.w0 == q.w1) x = a.lse[(int64_t)b * hq + kvh * a.group + 16 * g + c] * LOG2E;
+            else {
+                float L;
+                const float ref = stats(q, c, &L);
+                x = L == 0.f ? -INFINITY : ref + __log2f(L);
+            }
+            // no weight at all: every score is -inf, and so is every difference to a finite number
+            if (lane == 0) lse2[c] = x == -INFINITY ? 0.f : x;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int t = t0 + 256 * k + tid;
+            if (t < len) {
+                const float* s = a.scores + ((int64_t)(q.first + t / unit) * a.score_rows) * unit + t % unit;
+                for (int c = 0; c < nh; ++c) sum[k] += ex2(s[c * unit] - lse2[c]);
+            }
+        }
+        __syncthreads();
+    }
+    float* mass = a.mass + ((int64_t)b * p.heads + kvh) * a.side_ld;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int t = t0 + 256 * k + tid;
+        if (t < len) mass[t] += sum[k];
+    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -323,23 +731,80 @@ __global__ __launch_bounds__(256) void kv_move_kernel(const KvPool p, const KvTa
 
 }  // namespace
 
+// Compute units of a device, asked for once. (256 where the question fails, as it does without a GPU.)
+static int kv_cus(int device) {
+    static std::atomic<int> known[64];
+    if (device < 0 || device >= 64) return 256;
+    int n = known[device].load(std::memory_order_relaxed);
+    if (n) return n;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 1) {
+        (void)hipGetLastError();
+        return 256;
+    }
+    known[device].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hipStream_t s) {
     const int64_t copies = (int64_t)a.T * p.heads * ((p.dim * p.esize) >> 4);
     const bool side = a.mass || a.positions;
     kv_append_kernel<<<dim3((unsigned)((copies + 255) / 256), tb.B, side ? 3 : 2), 256, 0, s>>>(p, tb, a);
 }
 
-size_t kv_attend_ws_bytes(const KvPool&, int, int, int, bool) { return 0; }
+// Units of the line if every sequence filled its table.
+static int64_t attend_units(const KvPool& p, int B, int group, int max_pages) {
+    const int unit = attend_unit(p.dtype);
+    return (((int64_t)max_pages << p.page_shift) + unit - 1) / unit * B * p.heads * ((group + 15) / 16);
+}
 
-void launch_kv_attend(const KvPool& p, const KvTable& tb, const KvAttend& a, hipStream_t s) {
-    const dim3 grid(p.heads * a.group, tb.B), mgrid((((int64_t)tb.max_pages << p.page_shift) + 255) / 256, p.heads, tb.B);
-    if (p.dtype == KV_F32) kv_attend_kernel<float><<<grid, 256, 0, s>>>(p, tb, a);
-    else if (p.dtype == KV_BF16) kv_attend_kernel<bf16_t><<<grid, 256, 0, s>>>(p, tb, a);
-    else kv_attend_kernel<f16_t><<<grid, 256, 0, s>>>(p, tb, a);
-    if (!a.mass) return;
-    if (p.dtype == KV_F32) kv_mass_kernel<float><<<mgrid, 256, 0, s>>>(p, tb, a);
-    else if (p.dtype == KV_BF16) kv_mass_kernel<bf16_t><<<mgrid, 256, 0, s>>>(p, tb, a);
-    else kv_mass_kernel<f16_t><<<mgrid, 256, 0, s>>>(p, tb, a);
+bool kv_attend_fits(const KvPool& p, int B, int group, int max_pages) {
+    // units are counted in 31 bits on the device, workgroups of 256 threads in 32
+    const int64_t cap = (int64_t)max_pages << p.page_shift;
+    return attend_units(p, B, group, max_pages) < (1ll << 30) &&
+           (int64_t)B * p.heads * (group + (cap + MASS_TOKENS - 1) / MASS_TOKENS) < (1ll << 24);
+}
+
+// Workgroups of the attention: two to a CU keep enough loads in flight, and a unit each where there are fewer units.
+static int attend_shares(const KvPool& p, int B, int group, int max_pages) {
+    return (int)std::min<int64_t>(attend_units(p, B, group, max_pages), std::min(2 * kv_cus(p.device), AT_JOIN_MAX));
+}
+
+// {maximum, sum} and output of two parts per workgroup (the one it begins with, the one it ends with), and the scores
+size_t kv_attend_ws_bytes(const KvPool& p, int B, int group, int max_pages, bool mass) {
+    const size_t parts = 2 * (size_t)attend_shares(p, B, group, max_pages), rows = (size_t)std::min(group, 16);
+    size_t n = parts * 16 * sizeof(float2) + parts * rows * p.dim * sizeof(float);
+    if (mass) n += (size_t)attend_units(p, B, group, max_pages) * rows * attend_unit(p.dtype) * sizeof(float);
+    return n;
+}
+
+template <int DT, int D>
+static void attend_launch(const KvPool& p, const KvTable& tb, const KvAttend& a, int W, hipStream_t s) {
+    if (a.mass) kv_attend_kernel<DT, D, true><<<W, 256, 0, s>>>(p, tb, a);
+    else kv_attend_kernel<DT, D, false><<<W, 256, 0, s>>>(p, tb, a);
+}
+
+template <int D>
+static void attend_both(const KvPool& p, const KvTable& tb, const KvAttend& a, int W, hipStream_t s) {
+    if (p.dtype == KV_F32) attend_launch<KV_F32, D>(p, tb, a, W, s);
+    else if (p.dtype == KV_BF16) attend_launch<KV_BF16, D>(p, tb, a, W, s);
+    else attend_launch<KV_F16, D>(p, tb, a, W, s);
+    const int unit = attend_unit(p.dtype);
+    const int64_t cap = (int64_t)tb.max_pages << p.page_shift;
+    if (cap <= unit && !a.mass) return;              // nothing is ever in parts
+    int64_t blocks = (int64_t)tb.B * p.heads * a.group;
+    if (a.mass) blocks += (int64_t)tb.B * p.heads * ((cap + MASS_TOKENS - 1) / MASS_TOKENS);
+    kv_join_kernel<D><<<(unsigned)blocks, 256, 0, s>>>(p, tb, a, W, unit);
+}
+
+void launch_kv_attend(const KvPool& p, const KvTable& tb, KvAttend a, void* ws, hipStream_t s) {
+    const int W = attend_shares(p, tb.B, a.group, tb.max_pages);
+    a.score_rows = std::min(a.group, 16);
+    a.part_ml = (float2*)ws;
+    a.part_out = (float*)(a.part_ml + (size_t)2 * W * 16);
+    a.scores = a.part_out + (size_t)2 * W * a.score_rows * p.dim;
+    if (p.dim == 64) attend_both<64>(p, tb, a, W, s);
+    else if (p.dim == 128) attend_both<128>(p, tb, a, W, s);
+    else attend_both<256>(p, tb, a, W, s);
 }
 
 // Entries of one list: ranks of kept slots and numbers of gaps lie below n <= min(budget, capacity).
