@@ -264,7 +264,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
                 // a masked slot reads the pool's first row: its score is replaced
                 const char* r = good(tok, page[s]) ? kbase + page[s] * kp + (tok & mask) * kt : (const char*)p.k;
 #pragma unroll
-                for (int j = 0; j < KL; ++j) kf[s][j] = *reinterpret_cast<const u32x4*>(r + grp * 16 + j * 64);
+                for (int j = 0; j < KL; ++j) kf[s][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(r + grp * 16 + j * 64));
             }
         };
         int t = tile * UNIT + wave * TW;
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
                 for (int i = 0; i < 4; ++i) {
                     const char* r = ok[s] && tok + i < tend ? vbase + vpage[s] * vp + ((tok + i) & mask) * vt : (const char*)p.v;
 #pragma unroll
-                    for (int x = 0; x < NX; ++x) vf[4 * s + i][x] = *reinterpret_cast<const vload_t*>(r + (col + 16 * x) * VEC * ES);
+                    for (int x = 0; x < NX; ++x) vf[4 * s + i][x] = __builtin_nontemporal_load(reinterpret_cast<const vload_t*>(r + (col + 16 * x) * VEC * ES));
                 }
             }
             float sc[NV];
@@ -446,14 +446,24 @@ struct Parts {
     __device__ int slot(const Line& line, int w) const { return 2 * w + (line.begin(w) < first); }
 };
 
+// {reference exponent, sum} of two disjoint sets of weights as one.
+__device__ __forceinline__ float2 stat_join(float2 x, float2 y) {
+    const float M = fmaxf(x.x, y.x), ref = M == -INFINITY ? 0.f : M;
+    return float2{M, x.y * ex2(x.x - ref) + y.y * ex2(y.x - ref)};
+}
+
 // Workgroups 0 .. B * hq - 1: the parts of one (sequence, query head) joined. The rest: MASS_TOKENS tokens of
 // mass[b][h] += sum over the query heads of h of exp(score - lse), from the scores that kv_attend_kernel left. The lse of
-// a head in parts is computed by whoever needs it (a few values), so that both fit one launch.
+// a head in parts is computed by whoever needs it (a few values), so that both fit one launch. Short work that waits for
+// one dependent load after the other, so every step loads all it needs at once: a part's {exponent, sum} per lane, eight
+// rows of the parts' outputs per lane, four tokens of a head's scores per lane.
 template <int D>
 __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTable tb, const KvAttend a, int W, int unit) {
+    constexpr int COLS = D / 4, ROWS = 256 / COLS;   // a lane joins four dims of every ROWS-th part
     __shared__ float fac[AT_JOIN_MAX];
-    __shared__ float sums[256];
+    __shared__ f32x4 sums[ROWS][COLS];
     __shared__ float lse2[16];
+    __shared__ float2 wave_stat[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cap = tb.max_pages << p.page_shift;
     const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
@@ -490,45 +500,59 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         q.w1 = line.share_of(q.first + nb - 1);
         return q;
     };
-    // reference exponent and sum of head c of a group, over its parts: a wave's lanes take a part each
-    auto stats = [&](const Parts& q, int c, float* L) {
-        float M = -INFINITY, sum = 0.f;
-        for (int w = q.w0 + lane; w <= q.w1; w += 64) M = fmaxf(M, a.part_ml[q.slot(line, w) * 16 + c].x);
-        for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-        const float ref = M == -INFINITY ? 0.f : M;
-        for (int w = q.w0 + lane; w <= q.w1; w += 64) {
-            const float2 x = a.part_ml[q.slot(line, w) * 16 + c];
-            sum += x.y * ex2(x.x - ref);
-        }
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-        *L = sum;
-        return ref;
+    // {exponent, sum} of head c over parts from, from + step, ...: the caller's lanes together, then the wave's
+    auto stats = [&](const Parts& q, int c, int from, int step) {
+        float2 x = {-INFINITY, 0.f};
+        for (int w = q.w0 + from; w <= q.w1; w += step) x = stat_join(x, a.part_ml[q.slot(line, w) * 16 + c]);
+        for (int o = 32; o; o >>= 1) x = stat_join(x, float2{__shfl_xor(x.x, o), __shfl_xor(x.y, o)});
+        return x;
     };
     if (join) {
         const Parts q = parts_of(h0 >> 4);
         if (q.w0 == q.w1) return;
         const int c = h0 & 15, n = q.w1 - q.w0 + 1;
-        float L;
-        const float ref = stats(q, c, &L);
+        float2 x = stats(q, c, tid, 256);
+        if (lane == 0) wave_stat[wave] = x;
+        __syncthreads();
+        x = stat_join(stat_join(wave_stat[0], wave_stat[1]), stat_join(wave_stat[2], wave_stat[3]));
+        const float ref = x.x == -INFINITY ? 0.f : x.x, L = x.y;
         for (int i = tid; i < n; i += 256) fac[i] = ex2(a.part_ml[q.slot(line, q.w0 + i) * 16 + c].x - ref);
         __syncthreads();
-        const int d = tid % D, k = tid / D;
-        float o = 0.f;
-        for (int i = k; i < n; i += 256 / D) o += fac[i] * a.part_out[((int64_t)q.slot(line, q.w0 + i) * a.score_rows + c) * D + d];
-        sums[tid] = o;
+        const int d4 = tid % COLS, k = tid / COLS;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        const float* po = a.part_out + (int64_t)c * D + 4 * d4;
+        for (int i = k; i < n; i += 8 * ROWS) {
+            f32x4 v[8];
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = min(i + j * ROWS, n - 1);      // (a part beyond the last: the last again, times 0)
+                v[j] = *reinterpret_cast<const f32x4*>(po + (int64_t)q.slot(line, q.w0 + r) * a.score_rows * D);
+                f[j] = fac[r];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j * ROWS < n) o += v[j] * f[j];
+        }
+        sums[k][d4] = o;
         __syncthreads();
-        if (tid >= D) return;
-        for (int i = 1; i < 256 / D; ++i) o += sums[tid + i * D];
+        if (k) return;
+#pragma unroll
+        for (int i = 1; i < ROWS; ++i) o += sums[i][d4];
         o *= L == 0.f ? 0.f : 1.f / L;
         const int64_t head = (int64_t)b * hq + kvh * a.group + h0;
         if (tid == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
-        if (p.dtype == KV_F32) ((float*)a.out)[head * D + d] = o;
-        else if (p.dtype == KV_BF16) ((bf16_t*)a.out)[head * D + d] = (bf16_t)o;
-        else ((f16_t*)a.out)[head * D + d] = (f16_t)o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t at = head * D + 4 * d4 + e;
+            if (p.dtype == KV_F32) ((float*)a.out)[at] = o[e];
+            else if (p.dtype == KV_BF16) ((bf16_t*)a.out)[at] = (bf16_t)o[e];
+            else ((f16_t*)a.out)[at] = (f16_t)o[e];
+        }
         return;
     }
-    constexpr int PER = MASS_TOKENS / 256;
-    float sum[PER] = {};
+    const int t = t0 + 4 * tid;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     for (int g = 0; g < ngrp; ++g) {
         const Parts q = parts_of(g);
         const int nh = min(16, a.group - 16 * g);
@@ -536,30 +560,28 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
             float x;
             if (q.w0 == q.w1) x = a.lse[(int64_t)b * hq + kvh * a.group + 16 * g + c] * LOG2E;
             else {
-                float L;
-                const float ref = stats(q, c, &L);
-                x = L == 0.f ? -INFINITY : ref + __log2f(L);
+                const float2 st = stats(q, c, lane, 64);
+                x = st.y == 0.f ? -INFINITY : (st.x == -INFINITY ? 0.f : st.x) + __log2f(st.y);
             }
             // no weight at all: every score is -inf, and so is every difference to a finite number
             if (lane == 0) lse2[c] = x == -INFINITY ? 0.f : x;
         }
         __syncthreads();
+        if (t < len) {                               // (units are multiples of 4 tokens: four scores lie together)
+            const float* s = a.scores + (int64_t)(q.first + t / unit) * a.score_rows * unit + t % unit;
+#pragma unroll 4
+            for (int c = 0; c < nh; ++c) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(s + c * unit);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int t = t0 + 256 * k + tid;
-            if (t < len) {
-                const float* s = a.scores + ((int64_t)(q.first + t / unit) * a.score_rows) * unit + t % unit;
-                for (int c = 0; c < nh; ++c) sum[k] += ex2(s[c * unit] - lse2[c]);
+                for (int e = 0; e < 4; ++e) sum[e] += ex2(x[e] - lse2[c]);
             }
         }
         __syncthreads();
     }
-    float* mass = a.mass + ((int64_t)b * p.heads + kvh) * a.side_ld;
+    float* mass = a.mass + ((int64_t)b * p.heads + kvh) * a.side_ld + t;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int t = t0 + 256 * k + tid;
-        if (t < len) mass[t] += sum[k];
-    }
+    for (int e = 0; e < 4; ++e)
+        if (t + e < len) mass[e] += sum[e];
 }
 
 // ---------------------------------------------------------------------------------------
