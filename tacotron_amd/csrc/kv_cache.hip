@@ -92,10 +92,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvPool p, const Kv
 // 16 leaves columns idle: the matrix cores have the room, the reads of K and V are what counts).
 //   S^T = K Q^T: a lane of the A operand is a token (lane & 15) with 16 bytes of its row at 16 (lane >> 4) + 64 j; the
 //     order of the summed dimension is free as long as Q has the same, so both are plain 16-byte loads.
-//   O^T += V^T P^T: the C layout of S^T leaves lane (g = lane >> 4, head = lane & 15) with tokens 4 g + i of every 16, which
-//     is the B operand as it stands when the summed tokens are taken in that order. A lane loads VEC consecutive
-//     dims of each of those tokens, 16 lanes a whole row; for 16-bit types the 8 x VEC block it holds is
-//     transposed in registers (one v_perm per dword). No LDS, no barrier in the loop.
+//   O^T += V^T P^T: the C layout of S^T leaves lane (g = lane >> 4, head = lane & 15) with rows 4 g + i of every 16, which
+//     is the B operand as it stands when the summed tokens are taken in that order. Row r of 16-token block s of a
+//     tile is token 8 (r / 4) + 4 s + r % 4, so a lane's eight tokens are consecutive: they share a page (pages hold 8 or
+//     more), their scores leave in one piece. A lane loads VEC consecutive dims of each of its tokens, 16 lanes
+//     a whole row; for 16-bit types the 8 x VEC block it holds is transposed in registers (one v_perm per dword). No
+//     LDS, no barrier in the loop.
 // fp32 runs on v_mfma_f32_16x16x4_f32, 16-bit types on the 16x16x32 ones.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -184,7 +186,7 @@ template <int DT, int D, bool MASS>
 __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
     using S = AttendShape<DT, D>;
     constexpr int TW = S::TW, UNIT = S::UNIT, VEC = S::VEC, NX = S::NX, NACC = S::NACC, KL = S::KL, ES = S::ES;
-    constexpr int NS = TW / 16, NV = TW / 4;         // 16-token blocks; tokens a lane holds
+    constexpr int NS = TW / 16, NV = TW / 4;         // 16-token blocks; tokens a lane holds, NV (lane >> 4) and on
     // fp16 weights are kept 2^14 too large (the sums with them): at most 16384, and 2^-28 is still a normal number, so that
     // many small weights beside a large one are not lost
     constexpr float OFF = DT == KV_F16 ? 14.f : 0.f;
@@ -194,6 +196,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
+    const int ktok = NS == 2 ? 8 * (col >> 2) + (col & 3) : col;     // token of this lane's K row, block 0
     const int cap = tb.max_pages << p.page_shift, w = blockIdx.x, W = gridDim.x;
     const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
 
@@ -253,53 +256,41 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
 #pragma unroll
         for (int n = 0; n < NACC; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-        // page of slot t (t may lie behind the share: the last slot's then, masked later)
+        // page of slot t; of the share's last one where t lies behind it, so that every row below is in the pool (and
+        // of page 0 where the id is bad): what is masked is read and thrown away. A lane's NV tokens share a page.
         auto page_of = [&](int t) { return row[min(t, tend - 1) >> p.page_shift]; };
-        auto good = [&](int t, int page) { return t < tend && (unsigned)page < (unsigned)p.num_pages; };
+        auto bad_id = [&](int page) { return (unsigned)page >= (unsigned)p.num_pages; };
         u32x4 kf[NS][KL];
-        auto load_k = [&](int t, const int* page) {
+        auto load_k = [&](int t, int page) {
+            const char* r = kbase + (int64_t)(bad_id(page) ? 0 : page) * kp + ((t + ktok) & mask) * kt + grp * 16;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const int tok = t + 16 * s + col;
-                // a masked slot reads the pool's first row: its score is replaced
-                const char* r = good(tok, page[s]) ? kbase + page[s] * kp + (tok & mask) * kt : (const char*)p.k;
+            for (int s = 0; s < NS; ++s)
 #pragma unroll
-                for (int j = 0; j < KL; ++j) kf[s][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(r + grp * 16 + j * 64));
-            }
+                for (int j = 0; j < KL; ++j)
+                    kf[s][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(r + 4 * s * kt + j * 64));
         };
         int t = tile * UNIT + wave * TW;
-        int kpage[NS], vpage[NS];
+        int kpage = 0, vpage = 0;
         if (t < tend) {
-#pragma unroll
-            for (int s = 0; s < NS; ++s) { kpage[s] = page_of(t + 16 * s + col); vpage[s] = page_of(t + 16 * s + 4 * grp); }
+            kpage = page_of(t + ktok);
+            vpage = page_of(t + NV * grp);
             load_k(t, kpage);
-#pragma unroll
-            for (int s = 0; s < NS; ++s) kpage[s] = page_of(t + UNIT + 16 * s + col);
+            kpage = page_of(t + UNIT + ktok);
         }
         float* scores = nullptr;
-        if (MASS) scores = a.scores + ((int64_t)(u - tile) * a.score_rows + col) * UNIT + 4 * grp;
+        if (MASS) scores = a.scores + ((int64_t)(u - tile) * a.score_rows + col) * UNIT + wave * TW + NV * grp;
         for (; t < tend; t += UNIT) {
             // pages of the tile after the next, then V of this one: in flight during the first product
-            int kpage2[NS], vpage2[NS];
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                kpage2[s] = page_of(t + 2 * UNIT + 16 * s + col);
-                vpage2[s] = page_of(t + UNIT + 16 * s + 4 * grp);
-            }
+            const int kpage2 = page_of(t + 2 * UNIT + ktok), vpage2 = page_of(t + UNIT + NV * grp);
+            const int tok = t + NV * grp;
+            const bool bad = bad_id(vpage);
             vload_t vf[NV][NX];
-            bool ok[NS];
+            const char* r = vbase + (int64_t)(bad ? 0 : vpage) * vp + (tok & mask) * vt + col * VEC * ES;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const int tok = t + 16 * s + 4 * grp;
-                ok[s] = (unsigned)vpage[s] < (unsigned)p.num_pages;
-                if (!ok[s] && tok < tend) atomicOr(p.status, KV_BAD_PAGE);
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const char* r = ok[s] && tok + i < tend ? vbase + vpage[s] * vp + ((tok + i) & mask) * vt : (const char*)p.v;
-#pragma unroll
-                    for (int x = 0; x < NX; ++x) vf[4 * s + i][x] = __builtin_nontemporal_load(reinterpret_cast<const vload_t*>(r + (col + 16 * x) * VEC * ES));
-                }
-            }
+                for (int x = 0; x < NX; ++x)
+                    vf[i][x] = __builtin_nontemporal_load(reinterpret_cast<const vload_t*>(r + i * vt + x * 16 * VEC * ES));
             float sc[NV];
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
@@ -310,14 +301,12 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
                 for (int i = 0; i < 4; ++i) sc[4 * s + i] = c[i] * a.scale2;
             }
             if (t + UNIT < tend) load_k(t + UNIT, kpage);
-            bool all_ok = t + TW <= tend;
-#pragma unroll
-            for (int s = 0; s < NS; ++s) all_ok &= ok[s];
-            if (!__all(all_ok)) {
+            if (t + TW > tend || __any(bad)) {
                 // masked slots: score -inf, and no row that 0 could be multiplied with to give NaN
+                if (bad && tok < tend) atomicOr(p.status, KV_BAD_PAGE);
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
-                    if (!(ok[i >> 2] && t + 16 * (i >> 2) + 4 * grp + (i & 3) < tend)) {
+                    if (bad || tok + i >= tend) {
                         sc[i] = -INFINITY;
 #pragma unroll
                         for (int x = 0; x < NX; ++x) vf[i][x] = vload_t{};
@@ -326,7 +315,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
             if (MASS && col < nh) {
 #pragma unroll
                 for (int s = 0; s < NS; ++s)
-                    *reinterpret_cast<f32x4*>(scores + (int64_t)(t / UNIT) * a.score_rows * UNIT + wave * TW + 16 * s) =
+                    *reinterpret_cast<f32x4*>(scores + (int64_t)(t / UNIT) * a.score_rows * UNIT + 4 * s) =
                         f32x4{sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]};
             }
             float mx = sc[0];
@@ -371,8 +360,8 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
                         acc[x * VEC + e] = Mma<DT>::run(v, lo, acc[x * VEC + e]);
                     }
             }
-#pragma unroll
-            for (int s = 0; s < NS; ++s) { kpage[s] = kpage2[s]; vpage[s] = vpage2[s]; }
+            kpage = kpage2;
+            vpage = vpage2;
         }
 
         // the four waves' parts: wave r adds up component r of every accumulator, dims x 16 VEC + (4 grp + r) VEC + e
