@@ -274,7 +274,7 @@ struct KvAttend {
     void* out; float* lse;                // contiguous
     float* mass; int64_t side_ld;
     // workspace: parts of heads that several workgroups share, [2 * workgroups][16] {maximum, sum} and
-    // [2 * workgroups][score_rows][dim]; with mass, the scores, [units][score_rows][unit]
+    // [2 * workgroups][score_rows][dim]; with mass, the scores, [units][4 waves][score_rows][a wave's tokens]
     float2* part_ml; float* part_out; float* scores; int score_rows;
 };
 struct KvEvict {

@@ -119,6 +119,9 @@ struct AttendShape {
     static constexpr int NX = D / (16 * VEC);
     static constexpr int NACC = D / 16;
     static constexpr int KL = D * ES / 64;                     // 16-byte loads per lane and K row
+    // Floats of scores a wave gathers in LDS: two workgroups' tables fill a CU's 160 KB (one's at D = 256, whose registers
+    // allow no second)
+    static constexpr int GATHER = (D == 64 ? 16 : D == 128 ? 13 : 24) * 256;
 };
 
 int attend_unit(int dtype) { return dtype == KV_F32 ? AttendShape<KV_F32, 64>::UNIT : AttendShape<KV_BF16, 64>::UNIT; }
@@ -193,6 +196,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
     typedef typename std::conditional<VEC * ES == 16, u32x4, u32x2>::type vload_t;
     __shared__ float xch[4][3][NACC][64];            // quarter, source wave, accumulator, lane
     __shared__ float2 ml[AT_WAVES][16];
+    __shared__ f32x4 gathered[MASS ? AT_WAVES : 1][MASS ? S::GATHER / 4 : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
@@ -234,6 +238,21 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
     before = __builtin_amdgcn_readfirstlane(before);
     int nb = units_of(tb, a.lengths, b, cap, UNIT);
     int hg = (u0 - before) / nb, tile = (u0 - before) % nb;
+
+    // Scores for the weights of `mass`: [unit][wave][score_rows][TW]. A wave gathers those of its tiles of units gather0,
+    // gather0 + 1, ... and writes them out when there is room for no more, and at the end: a trickle of writes among the
+    // reads costs far more of the memory's time than their bytes.
+    const int tile_vecs = a.score_rows * TW / 4, room = S::GATHER / 4 / tile_vecs;
+    int gather0 = u0;
+    auto flush = [&](int upto) {
+        f32x4* to = (f32x4*)a.scores + ((int64_t)gather0 * AT_WAVES + wave) * tile_vecs;
+        const int n = min(upto - gather0, room);     // (units in which this wave had no tile may lie behind)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int i = 0; i < n; ++i, to += AT_WAVES * tile_vecs)
+            for (int j = lane; j < tile_vecs; j += 64) to[j] = gathered[wave][i * tile_vecs + j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        gather0 = upto;
+    };
 
     for (int u = u0; u < u1;) {
         const int stop = min(nb, tile + (u1 - u));
@@ -277,8 +296,6 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
             load_k(t, kpage);
             kpage = page_of(t + UNIT + ktok);
         }
-        float* scores = nullptr;
-        if (MASS) scores = a.scores + ((int64_t)(u - tile) * a.score_rows + col) * UNIT + wave * TW + NV * grp;
         for (; t < tend; t += UNIT) {
             // pages of the tile after the next, then V of this one: in flight during the first product
             const int kpage2 = page_of(t + 2 * UNIT + ktok), vpage2 = page_of(t + UNIT + NV * grp);
@@ -312,11 +329,14 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
                         for (int x = 0; x < NX; ++x) vf[i][x] = vload_t{};
                     }
             }
-            if (MASS && col < nh) {
+            if constexpr (MASS) {
+                const int unit = u - tile + t / UNIT;
+                if (unit - gather0 >= room) flush(unit);
+                if (col < nh) {
+                    f32x4* to = gathered[wave] + (unit - gather0) * tile_vecs + (col * TW + NV * grp) / 4;
 #pragma unroll
-                for (int s = 0; s < NS; ++s)
-                    *reinterpret_cast<f32x4*>(scores + (int64_t)(t / UNIT) * a.score_rows * UNIT + 4 * s) =
-                        f32x4{sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]};
+                    for (int s = 0; s < NS; ++s) to[s] = f32x4{sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]};
+                }
             }
             float mx = sc[0];
 #pragma unroll
@@ -427,6 +447,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
             }
         }
     }
+    if constexpr (MASS) flush(u1);
 }
 
 // Parts of one (sequence, head group): workgroups w0 .. w1, and where part w of them lies in the workspace.
@@ -556,11 +577,12 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
             if (lane == 0) lse2[c] = x == -INFINITY ? 0.f : x;
         }
         __syncthreads();
-        if (t < len) {                               // (units are multiples of 4 tokens: four scores lie together)
-            const float* s = a.scores + (int64_t)(q.first + t / unit) * a.score_rows * unit + t % unit;
+        if (t < len) {                               // (tiles are multiples of 4 tokens: four scores lie together)
+            const int tw = unit / AT_WAVES;
+            const float* s = a.scores + ((int64_t)q.first * AT_WAVES + t / tw) * a.score_rows * tw + t % tw;
 #pragma unroll 4
             for (int c = 0; c < nh; ++c) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(s + c * unit);
+                const f32x4 x = *reinterpret_cast<const f32x4*>(s + c * tw);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] += ex2(x[e] - lse2[c]);
             }
