@@ -607,42 +607,183 @@ __device__ __forceinline__ uint32_t mass_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Bits [shift, shift + bits) of the n-th greatest key, found from a histogram of the keys that agree with `prefix` above
-// them: the digit, and how many of the n are left to find below it.
-__device__ void pick_digit(const uint32_t* hist, int bins, int want, uint32_t* digit, int* left) {
-    // one wave walks the bins from the top, 64 at a time
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x;
-        int seen = 0;
-        for (int top = bins - 1; top >= 0; top -= 64) {
-            const int bin = top - lane;
-            int c = bin >= 0 ? (int)hist[bin] : 0;
-            int inc = c;
-            for (int o = 1; o < 64; o <<= 1) {
-                const int x = __shfl_up(inc, o);
-                if (lane >= o) inc += x;
-            }
-            const unsigned long long hit = __ballot(seen + inc >= want);
-            if (hit) {
-                const int at = __ffsll(hit) - 1;
-                if (lane == at) { *digit = (uint32_t)bin; *left = want - (seen + inc - c); }
-                break;
-            }
-            seen += __shfl(inc, 63);
-        }
+constexpr int EV_LIST = 4096;
+
+struct SelectShared {
+    uint32_t hist[2048];
+    uint32_t list[EV_LIST];                          // keys that agree with the threshold's first digit
+    int wave_a[EV_THREADS / 64], wave_b[EV_THREADS / 64];
+    uint32_t digit;
+    int left, same, listed, newest, kept_low;        // same: keys with the digit
+};
+
+// The greatest digit d of a histogram of 2048 bins with at least `want` keys at it or above, and how many of the want are
+// left for d itself. Two bins a thread, from the top; ends with a barrier.
+__device__ __forceinline__ void pick_digit(SelectShared& sh, int want) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, top = 2047 - 2 * tid;
+    const int c0 = (int)sh.hist[top], c1 = (int)sh.hist[top - 1];
+    int inc = c0 + c1;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(inc, o);
+        if (lane >= o) inc += x;
     }
+    if (lane == 63) sh.wave_a[wave] = inc;
+    __syncthreads();
+    for (int w = 0; w < EV_THREADS / 64; ++w) inc += w < wave ? sh.wave_a[w] : 0;
+    const int over = inc - c0 - c1;                  // keys above this thread's bins
+    if (over < want && want <= inc) {
+        const bool upper = over + c0 >= want;
+        sh.digit = (uint32_t)(upper ? top : top - 1);
+        sh.left = want - over - (upper ? 0 : c0);
+        sh.same = upper ? c0 : c1;
+    }
+    __syncthreads();
+}
+
+// f(i) for a wave's rows i < per, in register-sized groups (R > 0: i is a constant, up to a group's worth of rows behind
+// per are visited too) or one by one.
+template <int R, class F>
+__device__ __forceinline__ void for_rows(int per, F f) {
+    if constexpr (R == 0) {
+        for (int i = 0; i < per; ++i) f(i);
+    } else {
+        constexpr int G = R < 8 ? R : 8;
+#pragma unroll
+        for (int g = 0; g < R; g += G)
+            if (g < per) {
+#pragma unroll
+                for (int j = 0; j < G; ++j) f(g + j);
+                __builtin_amdgcn_sched_barrier(0);   // keeps one group's masks from living through all of them
+            }
+    }
+}
+
+// Kept slots of one head with len > n, see kv_select_kernel. A wave holds `per` rows of 64 consecutive slots, wave after
+// wave; R > 0: their keys in registers (per <= R), R = 0: read again in every pass.
+template <int R>
+__device__ __forceinline__ void select_head(SelectShared& sh, const KvEvict& a, int len, int n, const float* mass, const int32_t* pos,
+                            float* mass_out, int32_t* pos_out, int32_t* gaps, int32_t* late) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = (len + EV_THREADS - 1) / EV_THREADS, s0 = wave * per * 64 + lane;
+    const int stop = min(len, (wave + 1) * per * 64);        // slots of this wave
+    if (tid == 0) { sh.newest = -0x7fffffff - 1; sh.listed = 0; }
+    for (int i = tid; i < 2048; i += EV_THREADS) sh.hist[i] = 0;
+    __syncthreads();
+    if (a.recent > 0) {
+        int mine = -0x7fffffff - 1;
+#pragma unroll 8
+        for (int s = s0; s < stop; s += 64) mine = max(mine, pos[s]);
+        for (int o = 32; o; o >>= 1) mine = max(mine, __shfl_xor(mine, o));
+        if (lane == 0) atomicMax(&sh.newest, mine);
+        __syncthreads();
+    }
+    const int64_t border = a.recent > 0 ? (int64_t)sh.newest - a.recent : INT64_MAX;      // positions above it are protected
+    // the key of slot s, 0 (no key is) behind the wave's slots
+    auto load = [&](int s) {
+        const int t = min(s, len - 1);
+        uint32_t k = mass_key(mass[t]);
+        if (a.recent > 0 && (int64_t)pos[t] > border) k = 0xffffffffu;
+        return s < stop ? k : 0u;
+    };
+    uint32_t keys[R > 0 ? R : 1];
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) keys[i] = 0u;
+        for_rows<R>(per, [&](int i) { keys[i] = load(s0 + 64 * i); });
+    }
+    auto key = [&](int i) {
+        if constexpr (R > 0) return keys[i];
+        else return load(s0 + 64 * i);
+    };
+    uint32_t thr = 0;
+    int need = n;
+    bool listed = false;
+    for (int shift = 21, bits = 11; ; ) {
+        auto count = [&](uint32_t k) {
+            const bool in = k != 0u && ((uint64_t)k >> (shift + bits)) == ((uint64_t)thr >> (shift + bits));
+            const uint32_t digit = (k >> shift) & ((1u << bits) - 1);
+            const unsigned long long who = __ballot(in);
+            if (who) {
+                // equal keys side by side (fresh tokens, protected ones) would queue for one counter: one add for all
+                const uint32_t one = (uint32_t)__builtin_amdgcn_readlane((int)digit, __ffsll(who) - 1);
+                if (__ballot(in && digit == one) == who) {
+                    if (lane == 0) atomicAdd(&sh.hist[one], (uint32_t)__popcll(who));
+                } else if (in) atomicAdd(&sh.hist[digit], 1u);
+            }
+        };
+        if (listed) {
+            for (int i = tid; i - lane < sh.listed; i += EV_THREADS) count(i < sh.listed ? sh.list[i] : 0u);
+        } else for_rows<R>(per, [&](int i) { count(key(i)); });
+        __syncthreads();
+        pick_digit(sh, need);
+        thr |= sh.digit << shift;
+        need = sh.left;
+        if (shift == 0) break;
+        if (shift == 21 && sh.same <= EV_LIST) {
+            // few enough keys share the first digit to look at them alone from here on
+            for_rows<R>(per, [&](int i) {
+                const uint32_t k = key(i);
+                const bool in = k != 0u && k >> 21 == thr >> 21;
+                const unsigned long long who = __ballot(in);
+                if (who) {
+                    int at = 0;
+                    if (lane == 0) at = atomicAdd(&sh.listed, __popcll(who));
+                    at = __builtin_amdgcn_readfirstlane(at);
+                    if (in) sh.list[at + __popcll(who & ((1ull << lane) - 1))] = k;
+                }
+            });
+            listed = true;
+        }
+        for (int i = tid; i < 2048; i += EV_THREADS) sh.hist[i] = 0;
+        __syncthreads();
+        bits = min(11, shift);
+        shift -= bits;
+    }
+    // all with a key above thr are kept, and the first `need` of those at it
+    int gt = 0, eq = 0;
+    for_rows<R>(per, [&](int i) {
+        const uint32_t k = key(i);
+        gt += __popcll(__ballot(k > thr));
+        eq += __popcll(__ballot(k == thr));
+    });
+    if (lane == 0) { sh.wave_a[wave] = gt; sh.wave_b[wave] = eq; }
+    __syncthreads();
+    gt = eq = 0;                                     // before this row
+    for (int w = 0; w < EV_THREADS / 64; ++w) {
+        gt += w < wave ? sh.wave_a[w] : 0;
+        eq += w < wave ? sh.wave_b[w] : 0;
+    }
+    const unsigned long long low = (1ull << lane) - 1;
+    const bool copy = mass_out != mass, copy_pos = pos_out != pos;
+    for_rows<R>(per, [&](int i) {
+        const int s = s0 + 64 * i;
+        const uint32_t k = key(i);
+        const unsigned long long bg = __ballot(k > thr), be = __ballot(k == thr);
+        const int e = eq + __popcll(be & low), before = gt + __popcll(bg & low) + min(e, need);
+        const bool keep = k > thr || (k == thr && e < need);
+        gt += __popcll(bg);
+        eq += __popcll(be);
+        if (s >= stop) return;
+        if (s == n) sh.kept_low = before;
+        if (s < n) {
+            if (!keep) gaps[s - before] = s;
+            else {
+                if (copy) mass_out[s] = mass[s];
+                if (copy_pos) pos_out[s] = pos[s];
+            }
+        } else if (keep) late[before] = s;           // the move empties it
+        else { mass_out[s] = 0.f; pos_out[s] = -1; }
+    });
     __syncthreads();
 }
 
 // One workgroup per (sequence, kv head). The n-th greatest key by a radix select of 11 + 11 + 10 bits, then one pass in
 // slot order with a running count of the kept: a gap below n is the (slot - kept before it)-th, a kept slot from n on
-// has rank `kept before it`, so both lists come out ascending without a sort.
+// has rank `kept before it`, so both lists come out ascending without a sort. Up to 65536 tokens the keys stay in
+// registers, so masses and positions are read from memory once (positions twice) and what is left are LDS counters.
 __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, const KvTable tb, const KvEvict a) {
-    __shared__ uint32_t hist[2048];
-    __shared__ uint32_t digit;
-    __shared__ int left, newest, kept_low;
-    __shared__ int wave_gt[EV_THREADS / 64], wave_eq[EV_THREADS / 64];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ SelectShared sh;
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const int cap = tb.max_pages << p.page_shift;
     const int len = clamp_len(a.lengths[b], cap, p.status, h == 0 && tid == 0);
     const int n = min(len, a.budget);
@@ -653,77 +794,20 @@ __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, c
     int32_t* pos_out = a.positions_out + row * a.side_ld;
     int32_t* gaps = a.lists + row * 2 * a.list_ld;
     int32_t* late = gaps + a.list_ld;
-    uint32_t thr = 0;            // len <= budget: every key is kept
-    int need = 0;
-    if (tid == 0) { newest = -0x7fffffff - 1; kept_low = n; }
-    __syncthreads();
     if (len > n) {
-        int mine = -0x7fffffff - 1;
-        for (int s = tid; s < len; s += EV_THREADS) mine = max(mine, pos[s]);
-        for (int o = 32; o; o >>= 1) mine = max(mine, __shfl_xor(mine, o));
-        if (lane == 0) atomicMax(&newest, mine);
-        __syncthreads();
-    }
-    const int64_t border = (int64_t)newest - a.recent;      // positions above it are protected
-    auto key = [&](int s) { return (int64_t)pos[s] > border ? 0xffffffffu : mass_key(mass[s]); };
-    if (len > n && n > 0) {
-        need = n;
-        int shift = 32;
-        for (int bits = 11; shift > 0; ) {
-            if (shift < bits) bits = shift;
-            const uint32_t above = shift == 32 ? 0u : ~0u << shift;
-            shift -= bits;
-            for (int i = tid; i < 2048; i += EV_THREADS) hist[i] = 0;
-            __syncthreads();
-            for (int s = tid; s < len; s += EV_THREADS) {
-                const uint32_t k = key(s);
-                if ((k & above) == thr) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
-            }
-            __syncthreads();
-            pick_digit(hist, 1 << bits, need, &digit, &left);
-            thr |= digit << shift;
-            need = left;
-            __syncthreads();
+        if (len <= 4 * EV_THREADS) select_head<4>(sh, a, len, n, mass, pos, mass_out, pos_out, gaps, late);
+        else if (len <= 16 * EV_THREADS) select_head<16>(sh, a, len, n, mass, pos, mass_out, pos_out, gaps, late);
+        else if (len <= 64 * EV_THREADS) select_head<64>(sh, a, len, n, mass, pos, mass_out, pos_out, gaps, late);
+        else select_head<0>(sh, a, len, n, mass, pos, mass_out, pos_out, gaps, late);
+    } else {
+        for (int s = tid; s < len; s += EV_THREADS) {
+            if (mass_out != mass) mass_out[s] = mass[s];
+            if (pos_out != pos) pos_out[s] = pos[s];
         }
     }
-    // all with a key above thr are kept, and the first `need` of those at it
-    int gt0 = 0, eq0 = 0;        // before this stretch of slots
-    for (int s0 = 0; s0 < a.side_ld; s0 += EV_THREADS) {
-        const int s = s0 + tid;
-        bool gt = false, eq = false;
-        if (s < len) {
-            if (len == n) gt = true;
-            else if (n > 0) { const uint32_t k = key(s); gt = k > thr; eq = k == thr; }
-        }
-        int before = 0;
-        bool keep = gt;
-        if (len > n && s0 < len) {
-            const unsigned long long bg = __ballot(gt), be = __ballot(eq);
-            if (lane == 0) { wave_gt[wave] = __popcll(bg); wave_eq[wave] = __popcll(be); }
-            __syncthreads();
-            const unsigned long long low = (1ull << lane) - 1;
-            int g = gt0 + __popcll(bg & low), e = eq0 + __popcll(be & low);
-            for (int w = 0; w < EV_THREADS / 64; ++w) {
-                if (w < wave) { g += wave_gt[w]; e += wave_eq[w]; }
-                gt0 += wave_gt[w];
-                eq0 += wave_eq[w];
-            }
-            before = g + min(e, need);
-            keep = gt || (eq && e < need);
-            if (s == n) kept_low = before;
-            if (s < n && !keep) gaps[s - before] = s;
-            if (s >= n && keep) late[before] = s;
-            __syncthreads();
-        }
-        if (s < a.side_ld && !(keep && s >= n)) {
-            // slots that stay, and slots that end up empty; gaps and the slots that fill them belong to the move
-            if (s < n) { if (keep) { mass_out[s] = mass[s]; pos_out[s] = pos[s]; } }
-            else { mass_out[s] = 0.f; pos_out[s] = -1; }
-        }
-    }
-    __syncthreads();
+    for (int64_t s = len + tid; s < a.side_ld; s += EV_THREADS) { mass_out[s] = 0.f; pos_out[s] = -1; }
     if (tid == 0) {
-        a.counts[2 * row] = kept_low;
+        a.counts[2 * row] = len > n ? sh.kept_low : n;
         a.counts[2 * row + 1] = n;
     }
 }
