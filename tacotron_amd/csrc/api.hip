@@ -1804,7 +1804,8 @@ extern "C" int taco_kv_evict(const TacoKvPool* pool, const int32_t* table, int64
         return fail("%s: workspace too small (taco_kv_evict_workspace_bytes) or not on a 16-byte boundary", what);
     DeviceScope scope(pool->device);
     if (!scope.ok) return fail("%s: device %d is not available", what, pool->device);
-    KvEvict a{lengths, budget, recent, mass, positions, side_ld, lengths_out, mass_out, positions_out, nullptr, nullptr, 0};
+    KvEvict a{lengths, budget, recent, mass, positions, side_ld, lengths_out, mass_out, positions_out,
+              nullptr, nullptr, 0, nullptr, nullptr, nullptr};
     launch_kv_evict(p, t, a, ws, (hipStream_t)stream);
     return check_launch(what);
 }

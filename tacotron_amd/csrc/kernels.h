@@ -281,7 +281,8 @@ struct KvEvict {
     const int32_t* lengths; int budget, recent;
     const float* mass; const int32_t* positions; int64_t side_ld;
     int32_t* lengths_out; float* mass_out; int32_t* positions_out;
-    int32_t* counts; int32_t* lists; int64_t list_ld;      // workspace
+    int32_t* counts; int32_t* lists; int64_t list_ld;      // workspace, as the next line
+    int32_t* chunk_newest; uint32_t* chunk_hist; uint32_t* chunk_list;
 };
 void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hipStream_t s);
 bool kv_attend_fits(const KvPool& p, int B, int group, int max_pages);

@@ -598,30 +598,101 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
 // ---------------------------------------------------------------------------------------
 // evict
 
-constexpr int EV_THREADS = 1024;
+constexpr int EV_THREADS = 1024, EV_WAVES = EV_THREADS / 64;
+constexpr int EV_LIST = 4096;            // keys that are looked at again from LDS
+constexpr int EV_ROWS = 16;              // rows of 64 slots a wave holds in registers, at most
+constexpr int EV_CHUNK = 8192;           // slots per workgroup where several share a head
 
-// Order-preserving bits of a mass: NaN above everything, -0 as +0; protected slots above that.
+// Order-preserving bits of a mass: NaN above everything, -0 as +0; protected slots above that. Never 0.
 __device__ __forceinline__ uint32_t mass_key(float x) {
     if (x != x) return 0xfffffffeu;
     const uint32_t u = __float_as_uint(x + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int EV_LIST = 4096;
-
 struct SelectShared {
     uint32_t hist[2048];
-    uint32_t list[EV_LIST];                          // keys that agree with the threshold's first digit
-    int wave_a[EV_THREADS / 64], wave_b[EV_THREADS / 64];
+    uint32_t list[EV_LIST];
+    int wave_a[EV_WAVES], wave_b[EV_WAVES];
     uint32_t digit;
     int left, same, listed, newest, kept_low;        // same: keys with the digit
 };
 
-// The greatest digit d of a histogram of 2048 bins with at least `want` keys at it or above, and how many of the want are
-// left for d itself. Two bins a thread, from the top; ends with a barrier.
-__device__ __forceinline__ void pick_digit(SelectShared& sh, int want) {
+// One (sequence, kv head) as the select kernels see it.
+struct Head {
+    int len, n;
+    const float* mass; const int32_t* pos;
+    float* mass_out; int32_t* pos_out;
+    int32_t* gaps; int32_t* late; int32_t* counts;
+    int64_t border;                                  // positions above it are protected
+    bool recent;
+    __device__ Head(const KvPool& p, const KvTable& tb, const KvEvict& a, int h, int b, bool report) {
+        len = clamp_len(a.lengths[b], tb.max_pages << p.page_shift, p.status, report);
+        n = min(len, a.budget);
+        const int64_t row = (int64_t)b * p.heads + h;
+        mass = a.mass + row * a.side_ld;
+        pos = a.positions + row * a.side_ld;
+        mass_out = a.mass_out + row * a.side_ld;
+        pos_out = a.positions_out + row * a.side_ld;
+        gaps = a.lists + row * 2 * a.list_ld;
+        late = gaps + a.list_ld;
+        counts = a.counts + 2 * row;
+        recent = a.recent > 0;
+        border = INT64_MAX;
+    }
+    // the key of slot s, 0 from stop on
+    __device__ __forceinline__ uint32_t key(int s, int stop) const {
+        const int t = min(s, stop - 1);
+        uint32_t k = mass_key(mass[t]);
+        if (recent && (int64_t)pos[t] > border) k = 0xffffffffu;
+        return s < stop ? k : 0u;
+    }
+};
+
+// f(i) for rows i < per of a wave, i a constant, in groups of up to 8 (rows behind per up to a group's end too).
+template <int R, class F>
+__device__ __forceinline__ void for_rows(int per, F f) {
+    constexpr int G = R < 8 ? R : 8;
+#pragma unroll
+    for (int g = 0; g < R; g += G)
+        if (g < per) {
+#pragma unroll
+            for (int j = 0; j < G; ++j) f(g + j);
+            __builtin_amdgcn_sched_barrier(0);       // keeps one group's masks from living through all of them
+        }
+}
+
+// Counts a key's digit if `in`. Equal digits side by side (fresh tokens, protected ones) would queue for one counter: where
+// a wave has only one digit it adds once.
+__device__ __forceinline__ void count_digit(SelectShared& sh, bool in, uint32_t digit) {
+    const unsigned long long who = __ballot(in);
+    if (!who) return;
+    const uint32_t one = (uint32_t)__builtin_amdgcn_readlane((int)digit, __ffsll(who) - 1);
+    if (__ballot(in && digit == one) == who) {
+        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.hist[one], (uint32_t)__popcll(who));
+    } else if (in) atomicAdd(&sh.hist[digit], 1u);
+}
+
+__device__ __forceinline__ void clear_hist(SelectShared& sh) {
+    for (int i = threadIdx.x; i < 2048; i += EV_THREADS) sh.hist[i] = 0;
+}
+
+// Sum of x over the workgroup, for every thread. Two barriers; wave_a is free again behind the second.
+__device__ __forceinline__ int block_sum(SelectShared& sh, int x) {
+    x = wave_sum(x);
+    if ((threadIdx.x & 63) == 0) sh.wave_a[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = 0;
+    for (int w = 0; w < EV_WAVES; ++w) x += sh.wave_a[w];
+    __syncthreads();
+    return x;
+}
+
+// The greatest digit d of a histogram of 2048 bins with at least `want` keys at it or above (sh.digit), how many of the
+// want are left for d itself (sh.left), how many keys have it (sh.same). A thread brings the counts of bins
+// 2047 - 2 tid and 2046 - 2 tid. Ends with a barrier.
+__device__ __forceinline__ void pick_digit(SelectShared& sh, int want, int c0, int c1) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, top = 2047 - 2 * tid;
-    const int c0 = (int)sh.hist[top], c1 = (int)sh.hist[top - 1];
     int inc = c0 + c1;
     for (int o = 1; o < 64; o <<= 1) {
         const int x = __shfl_up(inc, o);
@@ -629,7 +700,7 @@ __device__ __forceinline__ void pick_digit(SelectShared& sh, int want) {
     }
     if (lane == 63) sh.wave_a[wave] = inc;
     __syncthreads();
-    for (int w = 0; w < EV_THREADS / 64; ++w) inc += w < wave ? sh.wave_a[w] : 0;
+    for (int w = 0; w < EV_WAVES; ++w) inc += w < wave ? sh.wave_a[w] : 0;
     const int over = inc - c0 - c1;                  // keys above this thread's bins
     if (over < want && want <= inc) {
         const bool upper = over + c0 >= want;
@@ -640,176 +711,243 @@ __device__ __forceinline__ void pick_digit(SelectShared& sh, int want) {
     __syncthreads();
 }
 
-// f(i) for a wave's rows i < per, in register-sized groups (R > 0: i is a constant, up to a group's worth of rows behind
-// per are visited too) or one by one.
-template <int R, class F>
-__device__ __forceinline__ void for_rows(int per, F f) {
-    if constexpr (R == 0) {
-        for (int i = 0; i < per; ++i) f(i);
-    } else {
-        constexpr int G = R < 8 ? R : 8;
+__device__ __forceinline__ void pick_digit(SelectShared& sh, int want) {
+    pick_digit(sh, want, (int)sh.hist[2047 - 2 * threadIdx.x], (int)sh.hist[2046 - 2 * threadIdx.x]);
+}
+
+// Digits two and three of the threshold. each(f) calls f(key) for all keys, 0 for none, in whole waves. sh.hist is clear.
+template <class E>
+__device__ __forceinline__ void pick_rest(SelectShared& sh, E each, uint32_t* thr, int* need) {
 #pragma unroll
-        for (int g = 0; g < R; g += G)
-            if (g < per) {
-#pragma unroll
-                for (int j = 0; j < G; ++j) f(g + j);
-                __builtin_amdgcn_sched_barrier(0);   // keeps one group's masks from living through all of them
-            }
+    for (int pass = 0; pass < 2; ++pass) {
+        const int shift = pass ? 0 : 10, bits = pass ? 10 : 11;
+        const uint32_t t = *thr;
+        each([&](uint32_t k) { count_digit(sh, k != 0u && k >> (shift + bits) == t >> (shift + bits), k >> shift & ((1u << bits) - 1)); });
+        __syncthreads();
+        pick_digit(sh, *need);
+        *thr |= sh.digit << shift;
+        *need = sh.left;
+        if (!pass) {
+            clear_hist(sh);
+            __syncthreads();
+        }
     }
 }
 
-// Kept slots of one head with len > n, see kv_select_kernel. A wave holds `per` rows of 64 consecutive slots, wave after
-// wave; R > 0: their keys in registers (per <= R), R = 0: read again in every pass.
-template <int R>
-__device__ __forceinline__ void select_head(SelectShared& sh, const KvEvict& a, int len, int n, const float* mass, const int32_t* pos,
-                            float* mass_out, int32_t* pos_out, int32_t* gaps, int32_t* late) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (len + EV_THREADS - 1) / EV_THREADS, s0 = wave * per * 64 + lane;
-    const int stop = min(len, (wave + 1) * per * 64);        // slots of this wave
-    if (tid == 0) { sh.newest = -0x7fffffff - 1; sh.listed = 0; }
-    for (int i = tid; i < 2048; i += EV_THREADS) sh.hist[i] = 0;
-    __syncthreads();
-    if (a.recent > 0) {
-        int mine = -0x7fffffff - 1;
+// Greatest position of slots from .. stop - 1 step 64 over the workgroup into sh.newest (set to the least before).
+__device__ __forceinline__ void newest_of(SelectShared& sh, const int32_t* pos, int from, int stop) {
+    int x = -0x7fffffff - 1;
 #pragma unroll 8
-        for (int s = s0; s < stop; s += 64) mine = max(mine, pos[s]);
-        for (int o = 32; o; o >>= 1) mine = max(mine, __shfl_xor(mine, o));
-        if (lane == 0) atomicMax(&sh.newest, mine);
-        __syncthreads();
-    }
-    const int64_t border = a.recent > 0 ? (int64_t)sh.newest - a.recent : INT64_MAX;      // positions above it are protected
-    // the key of slot s, 0 (no key is) behind the wave's slots
-    auto load = [&](int s) {
-        const int t = min(s, len - 1);
-        uint32_t k = mass_key(mass[t]);
-        if (a.recent > 0 && (int64_t)pos[t] > border) k = 0xffffffffu;
-        return s < stop ? k : 0u;
-    };
-    uint32_t keys[R > 0 ? R : 1];
-    if constexpr (R > 0) {
-#pragma unroll
-        for (int i = 0; i < R; ++i) keys[i] = 0u;
-        for_rows<R>(per, [&](int i) { keys[i] = load(s0 + 64 * i); });
-    }
-    auto key = [&](int i) {
-        if constexpr (R > 0) return keys[i];
-        else return load(s0 + 64 * i);
-    };
-    uint32_t thr = 0;
-    int need = n;
-    bool listed = false;
-    for (int shift = 21, bits = 11; ; ) {
-        auto count = [&](uint32_t k) {
-            const bool in = k != 0u && ((uint64_t)k >> (shift + bits)) == ((uint64_t)thr >> (shift + bits));
-            const uint32_t digit = (k >> shift) & ((1u << bits) - 1);
-            const unsigned long long who = __ballot(in);
-            if (who) {
-                // equal keys side by side (fresh tokens, protected ones) would queue for one counter: one add for all
-                const uint32_t one = (uint32_t)__builtin_amdgcn_readlane((int)digit, __ffsll(who) - 1);
-                if (__ballot(in && digit == one) == who) {
-                    if (lane == 0) atomicAdd(&sh.hist[one], (uint32_t)__popcll(who));
-                } else if (in) atomicAdd(&sh.hist[digit], 1u);
-            }
-        };
-        if (listed) {
-            for (int i = tid; i - lane < sh.listed; i += EV_THREADS) count(i < sh.listed ? sh.list[i] : 0u);
-        } else for_rows<R>(per, [&](int i) { count(key(i)); });
-        __syncthreads();
-        pick_digit(sh, need);
-        thr |= sh.digit << shift;
-        need = sh.left;
-        if (shift == 0) break;
-        if (shift == 21 && sh.same <= EV_LIST) {
-            // few enough keys share the first digit to look at them alone from here on
-            for_rows<R>(per, [&](int i) {
-                const uint32_t k = key(i);
-                const bool in = k != 0u && k >> 21 == thr >> 21;
-                const unsigned long long who = __ballot(in);
-                if (who) {
-                    int at = 0;
-                    if (lane == 0) at = atomicAdd(&sh.listed, __popcll(who));
-                    at = __builtin_amdgcn_readfirstlane(at);
-                    if (in) sh.list[at + __popcll(who & ((1ull << lane) - 1))] = k;
-                }
-            });
-            listed = true;
-        }
-        for (int i = tid; i < 2048; i += EV_THREADS) sh.hist[i] = 0;
-        __syncthreads();
-        bits = min(11, shift);
-        shift -= bits;
-    }
-    // all with a key above thr are kept, and the first `need` of those at it
-    int gt = 0, eq = 0;
-    for_rows<R>(per, [&](int i) {
-        const uint32_t k = key(i);
-        gt += __popcll(__ballot(k > thr));
-        eq += __popcll(__ballot(k == thr));
-    });
-    if (lane == 0) { sh.wave_a[wave] = gt; sh.wave_b[wave] = eq; }
+    for (int s = from; s < stop; s += 64) x = max(x, pos[s]);
+    for (int o = 32; o; o >>= 1) x = max(x, __shfl_xor(x, o));
+    if ((threadIdx.x & 63) == 0) atomicMax(&sh.newest, x);
     __syncthreads();
-    gt = eq = 0;                                     // before this row
-    for (int w = 0; w < EV_THREADS / 64; ++w) {
+}
+
+// The outcome for a workgroup's slots: waves one after the other, `per` rows of 64 each from slot0 on, below stop. gt, eq:
+// keys above the threshold and at it in the slots before slot0. All above it are kept and the first `need` at it. A gap
+// below n is the (slot - kept before it)-th, a kept slot from n on has rank `kept before it`: both lists come out
+// ascending without a sort.
+template <int R>
+__device__ __forceinline__ void emit(SelectShared& sh, const Head& a, const uint32_t* keys, int slot0, int per, int stop, uint32_t thr,
+                                     int need, int gt, int eq) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int g = 0, e0 = 0;
+    for_rows<R>(per, [&](int i) {
+        g += __popcll(__ballot(keys[i] > thr));
+        e0 += __popcll(__ballot(keys[i] == thr));
+    });
+    if (lane == 0) { sh.wave_a[wave] = g; sh.wave_b[wave] = e0; }
+    __syncthreads();
+    for (int w = 0; w < EV_WAVES; ++w) {
         gt += w < wave ? sh.wave_a[w] : 0;
         eq += w < wave ? sh.wave_b[w] : 0;
     }
     const unsigned long long low = (1ull << lane) - 1;
-    const bool copy = mass_out != mass, copy_pos = pos_out != pos;
+    const bool copy = a.mass_out != a.mass, copy_pos = a.pos_out != a.pos;
     for_rows<R>(per, [&](int i) {
-        const int s = s0 + 64 * i;
-        const uint32_t k = key(i);
+        const int s = slot0 + (wave * per + i) * 64 + lane;
+        const uint32_t k = keys[i];
         const unsigned long long bg = __ballot(k > thr), be = __ballot(k == thr);
         const int e = eq + __popcll(be & low), before = gt + __popcll(bg & low) + min(e, need);
         const bool keep = k > thr || (k == thr && e < need);
         gt += __popcll(bg);
         eq += __popcll(be);
-        if (s >= stop) return;
-        if (s == n) sh.kept_low = before;
-        if (s < n) {
-            if (!keep) gaps[s - before] = s;
+        if (k == 0u) return;
+        if (s == a.n) a.counts[0] = before;
+        if (s < a.n) {
+            if (!keep) a.gaps[s - before] = s;
             else {
-                if (copy) mass_out[s] = mass[s];
-                if (copy_pos) pos_out[s] = pos[s];
+                if (copy) a.mass_out[s] = a.mass[s];
+                if (copy_pos) a.pos_out[s] = a.pos[s];
             }
-        } else if (keep) late[before] = s;           // the move empties it
-        else { mass_out[s] = 0.f; pos_out[s] = -1; }
+        } else if (keep) a.late[before] = s;         // the move empties it
+        else { a.mass_out[s] = 0.f; a.pos_out[s] = -1; }
     });
+}
+
+// Slots from .. to - 1 of a head that keeps what it has, and emptiness behind its length.
+__device__ __forceinline__ void keep_all(const Head& a, int64_t from, int64_t to) {
+    for (int64_t s = from + threadIdx.x; s < to; s += EV_THREADS) {
+        if (s >= a.len) { a.mass_out[s] = 0.f; a.pos_out[s] = -1; }
+        else if (a.len == a.n) {
+            if (a.mass_out != a.mass) a.mass_out[s] = a.mass[s];
+            if (a.pos_out != a.pos) a.pos_out[s] = a.pos[s];
+        }
+    }
+    if (from == 0 && threadIdx.x == 0) {
+        if (a.len == a.n) a.counts[0] = a.n;
+        a.counts[1] = a.n;
+    }
+}
+
+// A head of one workgroup: a wave holds `per` rows of 64 consecutive slots, their keys in registers.
+template <int R>
+__device__ __forceinline__ void select_head(SelectShared& sh, Head& a, int recent) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = (a.len + EV_THREADS - 1) / EV_THREADS, s0 = wave * per * 64 + lane;
+    const int stop = min(a.len, (wave + 1) * per * 64);        // slots of this wave
+    if (tid == 0) { sh.newest = -0x7fffffff - 1; sh.listed = 0; }
+    clear_hist(sh);
     __syncthreads();
+    if (a.recent) {
+        newest_of(sh, a.pos, s0, stop);
+        a.border = (int64_t)sh.newest - recent;
+    }
+    uint32_t keys[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) keys[i] = 0u;
+    if (wave * per * 64 < a.len) for_rows<R>(per, [&](int i) { keys[i] = i < per ? a.key(s0 + 64 * i, stop) : 0u; });
+    for_rows<R>(per, [&](int i) { count_digit(sh, keys[i] != 0u, keys[i] >> 21); });
+    __syncthreads();
+    pick_digit(sh, a.n);
+    uint32_t thr = sh.digit << 21;
+    int need = sh.left;
+    const bool few = sh.same <= EV_LIST;
+    clear_hist(sh);
+    if (few) {
+        // few enough keys share the first digit to look at them alone from here on
+        for_rows<R>(per, [&](int i) {
+            const bool in = keys[i] != 0u && keys[i] >> 21 == thr >> 21;
+            const unsigned long long who = __ballot(in);
+            if (who) {
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&sh.listed, __popcll(who));
+                at = __builtin_amdgcn_readfirstlane(at);
+                if (in) sh.list[at + __popcll(who & ((1ull << lane) - 1))] = keys[i];
+            }
+        });
+    }
+    __syncthreads();
+    if (few)
+        pick_rest(sh, [&](auto f) { for (int i = tid; i - lane < sh.listed; i += EV_THREADS) f(i < sh.listed ? sh.list[i] : 0u); }, &thr, &need);
+    else pick_rest(sh, [&](auto f) { for_rows<R>(per, [&](int i) { f(keys[i]); }); }, &thr, &need);
+    emit<R>(sh, a, keys, 0, per, stop, thr, need, 0, 0);
 }
 
 // One workgroup per (sequence, kv head). The n-th greatest key by a radix select of 11 + 11 + 10 bits, then one pass in
-// slot order with a running count of the kept: a gap below n is the (slot - kept before it)-th, a kept slot from n on
-// has rank `kept before it`, so both lists come out ascending without a sort. Up to 65536 tokens the keys stay in
-// registers, so masses and positions are read from memory once (positions twice) and what is left are LDS counters.
+// slot order. The keys stay in registers, so masses are read once and positions twice; what is left are LDS counters.
 __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, const KvTable tb, const KvEvict a) {
     __shared__ SelectShared sh;
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const int cap = tb.max_pages << p.page_shift;
-    const int len = clamp_len(a.lengths[b], cap, p.status, h == 0 && tid == 0);
-    const int n = min(len, a.budget);
-    const int64_t row = (int64_t)b * p.heads + h;
-    const float* mass = a.mass + row * a.side_ld;
-    const int32_t* pos = a.positions + row * a.side_ld;
-    float* mass_out = a.mass_out + row * a.side_ld;
-    int32_t* pos_out = a.positions_out + row * a.side_ld;
-    int32_t* gaps = a.lists + row * 2 * a.list_ld;
-    int32_t* late = gaps + a.list_ld;
-    if (len > n) {
-        if (len <= 4 * EV_THREADS) select_head<4>(sh, a, len, n, mass, pos, mass_out, pos_out, gaps, late);
-        else if (len <= 16 * EV_THREADS) select_head<16>(sh, a, len, n, mass, pos, mass_out, pos_out, gaps, late);
-        else if (len <= 64 * EV_THREADS) select_head<64>(sh, a, len, n, mass, pos, mass_out, pos_out, gaps, late);
-        else select_head<0>(sh, a, len, n, mass, pos, mass_out, pos_out, gaps, late);
-    } else {
-        for (int s = tid; s < len; s += EV_THREADS) {
-            if (mass_out != mass) mass_out[s] = mass[s];
-            if (pos_out != pos) pos_out[s] = pos[s];
+    Head head(p, tb, a, blockIdx.x, blockIdx.y, blockIdx.x == 0 && threadIdx.x == 0);
+    if (head.len > head.n) {
+        if (head.len <= 4 * EV_THREADS) select_head<4>(sh, head, a.recent);
+        else select_head<EV_ROWS>(sh, head, a.recent);
+    }
+    keep_all(head, 0, a.side_ld);
+}
+
+// The same for tables of more slots than a workgroup holds: a workgroup per chunk, four launches. Each workgroup works out
+// the head's threshold for itself from what the one before left: the chunks' newest positions, the chunks' histograms of the
+// first digit, the chunks' lists of the keys that share the threshold's first digit. Sums over chunks before
+// its own give it the ranks of its slots, so nothing waits for anything and no counter is shared.
+struct ChunkWork {
+    int32_t* newest;                     // [chunks]
+    uint32_t* hist;                      // [chunks][2048]
+    uint32_t* list;                      // [chunks][EV_CHUNK]
+    __device__ ChunkWork(const KvEvict& a, int64_t row, int chunks) {
+        newest = a.chunk_newest + row * chunks;
+        hist = a.chunk_hist + row * chunks * 2048;
+        list = a.chunk_list + row * chunks * EV_CHUNK;
+    }
+};
+
+// STAGE 0: newest position; 1: histogram; 2: list; 3: the outcome.
+template <int STAGE>
+__global__ __launch_bounds__(EV_THREADS) void kv_select_chunk_kernel(const KvPool p, const KvTable tb, const KvEvict a) {
+    constexpr int R = EV_CHUNK / EV_THREADS;
+    __shared__ SelectShared sh;
+    const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    Head head(p, tb, a, h, b, STAGE == 3 && c == 0 && h == 0 && tid == 0);
+    const ChunkWork ws(a, (int64_t)b * p.heads + h, gridDim.x);
+    const int slot0 = c * EV_CHUNK, s0 = slot0 + wave * (EV_CHUNK / EV_WAVES) + lane;
+    const int stop = min(head.len, slot0 + (wave + 1) * (EV_CHUNK / EV_WAVES));
+    const int chunks = (head.len + EV_CHUNK - 1) / EV_CHUNK;
+    if (STAGE == 3) keep_all(head, slot0, c + 1 == (int)gridDim.x ? a.side_ld : min<int64_t>(a.side_ld, slot0 + EV_CHUNK));
+    if (head.len <= head.n || c >= chunks) return;
+    if (tid == 0) { sh.newest = -0x7fffffff - 1; sh.listed = 0; }
+    clear_hist(sh);
+    __syncthreads();
+    if (STAGE == 0) {
+        newest_of(sh, head.pos, s0, stop);
+        if (tid == 0) ws.newest[c] = sh.newest;
+        return;
+    }
+    if (head.recent) {
+        newest_of(sh, ws.newest, tid, wave == 0 ? chunks : 0);
+        head.border = (int64_t)sh.newest - a.recent;
+    }
+    uint32_t keys[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) keys[i] = s0 - lane < stop ? head.key(s0 + 64 * i, stop) : 0u;
+    if (STAGE == 1) {
+        for_rows<R>(R, [&](int i) { count_digit(sh, keys[i] != 0u, keys[i] >> 21); });
+        __syncthreads();
+        for (int i = tid; i < 2048; i += EV_THREADS) ws.hist[(int64_t)c * 2048 + i] = sh.hist[i];
+        return;
+    }
+    // first digit, from the sum of the chunks' histograms
+    const int top = 2047 - 2 * tid;
+    int c0 = 0, c1 = 0, l0 = 0, l1 = 0;              // of all chunks, and of those before this one
+#pragma unroll 4
+    for (int i = 0; i < chunks; ++i) {
+        const uint2 x = *reinterpret_cast<const uint2*>(ws.hist + (int64_t)i * 2048 + top - 1);
+        c0 += (int)x.y;
+        c1 += (int)x.x;
+        l0 += i < c ? (int)x.y : 0;
+        l1 += i < c ? (int)x.x : 0;
+    }
+    pick_digit(sh, head.n, c0, c1);
+    const uint32_t digit = sh.digit;
+    if (STAGE == 2) {
+        for_rows<R>(R, [&](int i) {
+            const bool in = keys[i] != 0u && keys[i] >> 21 == digit;
+            const unsigned long long who = __ballot(in);
+            if (who) {
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&sh.listed, __popcll(who));
+                at = __builtin_amdgcn_readfirstlane(at);
+                if (in) ws.list[(int64_t)c * EV_CHUNK + at + __popcll(who & ((1ull << lane) - 1))] = keys[i];
+            }
+        });
+        return;
+    }
+    uint32_t thr = digit << 21;
+    int need = sh.left;
+    int gt = block_sum(sh, (top > (int)digit ? l0 : 0) + (top - 1 > (int)digit ? l1 : 0));
+    // the keys that share it, chunk by chunk
+    auto each = [&](int upto, auto f) {
+        for (int i = 0; i < upto; ++i) {
+            const int n = (int)ws.hist[(int64_t)i * 2048 + digit];
+            for (int j = tid; j - lane < n; j += EV_THREADS) f(j < n ? ws.list[(int64_t)i * EV_CHUNK + j] : 0u);
         }
-    }
-    for (int64_t s = len + tid; s < a.side_ld; s += EV_THREADS) { mass_out[s] = 0.f; pos_out[s] = -1; }
-    if (tid == 0) {
-        a.counts[2 * row] = len > n ? sh.kept_low : n;
-        a.counts[2 * row + 1] = n;
-    }
+    };
+    pick_rest(sh, [&](auto f) { each(chunks, f); }, &thr, &need);
+    int g = 0, e = 0;
+    each(c, [&](uint32_t k) { g += k > thr; e += k == thr; });
+    gt += block_sum(sh, g);
+    const int eq = block_sum(sh, e);
+    emit<R>(sh, head, keys, slot0, EV_CHUNK / EV_THREADS, stop, thr, need, gt, eq);
 }
 
 // Row late[kept_low + i] -> row gaps[i], K and V and the side tables. Sources lie at n and beyond, targets below it.
@@ -929,16 +1067,35 @@ static size_t kv_evict_list(const KvPool& p, int max_pages, int budget) {
     return (size_t)std::min<int64_t>(budget, (int64_t)max_pages << p.page_shift);
 }
 
-// gaps and late kept slots of every (sequence, kv head), and {kept below n, n}
+// Chunks of the long select, 0 where a workgroup holds a head. (One launch against four: an eviction of 32 heads takes 30
+// us and 45 at 8192 slots, 39 and 45 at 16384; at 65536 a workgroup a head took 168, the chunks 79.)
+static int64_t kv_evict_chunks(const KvPool& p, int max_pages) {
+    const int64_t cap = (int64_t)max_pages << p.page_shift;
+    return cap <= EV_ROWS * EV_THREADS ? 0 : (cap + EV_CHUNK - 1) / EV_CHUNK;
+}
+
+// {kept below n, n} of every (sequence, kv head), its gaps and late kept slots, and the chunks' tables
 size_t kv_evict_ws_bytes(const KvPool& p, int B, int max_pages, int budget) {
-    return (size_t)B * p.heads * (2 * kv_evict_list(p, max_pages, budget) + 2) * sizeof(int32_t);
+    return (size_t)B * p.heads * (2 * kv_evict_list(p, max_pages, budget) + 2 + kv_evict_chunks(p, max_pages) * (2 + 2048 + EV_CHUNK)) * 4;
 }
 
 void launch_kv_evict(const KvPool& p, const KvTable& tb, KvEvict a, void* ws, hipStream_t s) {
-    a.counts = (int32_t*)ws;
-    a.lists = a.counts + (size_t)2 * tb.B * p.heads;
+    const size_t rows = (size_t)tb.B * p.heads;
+    const int chunks = (int)kv_evict_chunks(p, tb.max_pages);
+    // 8-byte pairs of histogram bins first, everything else is read by the word
+    a.chunk_hist = (uint32_t*)ws;
+    a.chunk_list = a.chunk_hist + rows * chunks * 2048;
+    a.counts = (int32_t*)(a.chunk_list + rows * chunks * EV_CHUNK);
+    a.lists = a.counts + 2 * rows;
     a.list_ld = (int64_t)kv_evict_list(p, tb.max_pages, a.budget);
-    kv_select_kernel<<<dim3(p.heads, tb.B), EV_THREADS, 0, s>>>(p, tb, a);
+    a.chunk_newest = a.lists + 2 * rows * a.list_ld;
+    if (chunks) {
+        const dim3 grid(chunks, p.heads, tb.B);
+        if (a.recent > 0) kv_select_chunk_kernel<0><<<grid, EV_THREADS, 0, s>>>(p, tb, a);
+        kv_select_chunk_kernel<1><<<grid, EV_THREADS, 0, s>>>(p, tb, a);
+        kv_select_chunk_kernel<2><<<grid, EV_THREADS, 0, s>>>(p, tb, a);
+        kv_select_chunk_kernel<3><<<grid, EV_THREADS, 0, s>>>(p, tb, a);
+    } else kv_select_kernel<<<dim3(p.heads, tb.B), EV_THREADS, 0, s>>>(p, tb, a);
     const int64_t most = std::min((int64_t)a.budget, ((int64_t)tb.max_pages << p.page_shift) - a.budget);
     const int64_t vecs = std::max<int64_t>(most, 1) * ((p.dim * p.esize) >> 4);
     kv_move_kernel<<<dim3((unsigned)std::min<int64_t>((vecs + 255) / 256, 64), p.heads, tb.B), 256, 0, s>>>(p, tb, a);
