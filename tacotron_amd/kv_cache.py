@@ -50,6 +50,8 @@ class KvCache:
         p.k_page_stride, p.k_head_stride, p.k_token_stride = k_pages.stride()[:3]
         p.v_page_stride, p.v_head_stride, p.v_token_stride = v_pages.stride()[:3]
         self._pool, self._ref = p, ctypes.byref(p)
+        self._esize = k_pages.element_size()
+        self._need = {}
         # the library's own checks of the geometry, now and not at the first call
         if not self.lib.taco_kv_evict_workspace_bytes(self._ref, 1, 1, 1):
             raise TacoError(_lib.last_error())
@@ -76,34 +78,53 @@ class KvCache:
         if rc != 0:
             raise TacoError(_lib.last_error())
 
-    def _ints(self, t, name, shape):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device or t.shape != shape:
-            raise TacoError('%s must be an int32 tensor %s on %s' % (name, list(shape), self.device))
+    def _ints(self, t, name, B):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or t.shape[0] != B:
+            raise TacoError('%s must be an int32 tensor [%d] on %s' % (name, B, self.device))
         return t if t.is_contiguous() else t.contiguous()
 
-    def _table(self, t):
+    def _table(self, t, B=None):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device or t.dim() != 2 or not t.numel():
             raise TacoError('page_table must be an int32 tensor [B, max_pages] on %s' % self.device)
+        if B is not None and t.shape[0] != B:
+            raise TacoError('page_table must have a row for each of the %d sequences' % B)
         return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
     def _side(self, t, name, dtype, B, slots):
-        if (not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != self.device or t.dim() != 3 or
-                t.shape[0] != B or t.shape[1] != self.kv_heads or t.shape[2] < slots or not t.is_contiguous()):
-            raise TacoError('%s must be a contiguous %s tensor [%d, %d, at least %d] on %s'
-                            % (name, str(dtype)[6:], B, self.kv_heads, slots, self.device))
-        return t
+        if isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == self.device and t.dim() == 3 and t.is_contiguous():
+            n, h, ld = t.shape
+            if n == B and h == self.kv_heads and ld >= slots:
+                return ld
+        raise TacoError('%s must be a contiguous %s tensor [%d, %d, at least %d] on %s'
+                        % (name, str(dtype)[6:], B, self.kv_heads, slots, self.device))
 
     def _rows(self, t, name):
-        """Rows of head_dim elements: contiguous, 16-byte aligned, or copied to be."""
+        """Rows of head_dim elements: contiguous, 16-byte aligned, or copied to be. Returns it and its strides."""
         if t.dtype != self.dtype or t.device != self.device:
             raise TacoError('%s must be %s on %s, as the pool' % (name, str(self.dtype)[6:], self.device))
-        st, unit = t.stride(), 16 // t.element_size()
-        if st[-1] != 1 or t.data_ptr() % 16 or any(s % unit for s in st[:-1]):
-            return t.clone(memory_format=torch.contiguous_format)
-        return t
+        st = t.stride()
+        bits = t.data_ptr()
+        for s in st[:-1]:
+            bits |= s * self._esize
+        if st[-1] != 1 or bits & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+            st = t.stride()
+        return t, st
+
+    def _workspace(self, query, *sizes):
+        """Scratch of one call, from torch's allocator. Its size depends on the sizes alone and is asked for once."""
+        need = self._need.get((query, sizes))
+        if need is None:
+            need = getattr(self.lib, query)(self._ref, *sizes)
+            if not need:
+                raise TacoError(_lib.last_error())
+            if len(self._need) >= 256:
+                self._need.clear()
+            self._need[(query, sizes)] = need
+        return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     # ---- the operators
     def append(self, k, v, page_table, starts, counts=None, first=None, mass=None, positions=None):
@@ -116,25 +137,23 @@ class KvCache:
         if k.shape != v.shape:
             raise TacoError('k and v must have the same shape')
         B, T = k.shape[:2]
-        k, v, table = self._rows(k, 'k'), self._rows(v, 'v'), self._table(page_table)
-        if table.shape[0] != B:
-            raise TacoError('page_table must have a row for each of the %d sequences' % B)
-        slots = table.shape[1] * self.page_size
-        starts = self._ints(starts, 'starts', (B,))
-        counts = self._ints(counts, 'counts', (B,)) if counts is not None else None
-        first = self._ints(first, 'first', (B,)) if first is not None else None
-        ld = slots
+        (k, ks), (v, vs), table = self._rows(k, 'k'), self._rows(v, 'v'), self._table(page_table, B)
+        max_pages = table.shape[1]
+        ld = slots = max_pages * self.page_size
+        starts = self._ints(starts, 'starts', B)
+        counts = self._ints(counts, 'counts', B) if counts is not None else None
+        first = self._ints(first, 'first', B) if first is not None else None
         if mass is not None:
-            ld = self._side(mass, 'mass', torch.float32, B, slots).shape[2]
+            ld = self._side(mass, 'mass', torch.float32, B, slots)
         if positions is not None:
-            self._side(positions, 'positions', torch.int32, B, slots)
-            if mass is not None and positions.shape[2] != ld:
+            pos_ld = self._side(positions, 'positions', torch.int32, B, slots)
+            if mass is not None and pos_ld != ld:
                 raise TacoError('mass and positions must have the same shape')
-            ld = positions.shape[2]
+            ld = pos_ld
         lengths = torch.empty(B, dtype=torch.int32, device=self.device)
         self._check(self.lib.taco_kv_append(
-            self._ref, table.data_ptr(), table.stride(0), B, table.shape[1],
-            k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), T,
+            self._ref, table.data_ptr(), table.stride(0), B, max_pages,
+            k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], T,
             starts.data_ptr(), counts.data_ptr() if counts is not None else None,
             first.data_ptr() if first is not None else None, mass.data_ptr() if mass is not None else None,
             positions.data_ptr() if positions is not None else None, ld, lengths.data_ptr(), self._stream()))
@@ -148,24 +167,19 @@ class KvCache:
         gives out 0, lse -inf."""
         if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.shape[2] != self.head_dim or not q.numel():
             raise TacoError('q must be [B, q_heads, %d]' % self.head_dim)
-        B, hq = q.shape[:2]
-        q, table = self._rows(q, 'q'), self._table(page_table)
-        if table.shape[0] != B:
-            raise TacoError('page_table must have a row for each of the %d sequences' % B)
+        B, hq, _ = q.shape
+        (q, qs), table = self._rows(q, 'q'), self._table(page_table, B)
         max_pages = table.shape[1]
-        lengths = self._ints(lengths, 'lengths', (B,))
+        lengths = self._ints(lengths, 'lengths', B)
         ld = 0
         if mass is not None:
-            ld = self._side(mass, 'mass', torch.float32, B, max_pages * self.page_size).shape[2]
-        need = self.lib.taco_kv_attend_workspace_bytes(self._ref, B, hq, max_pages, mass is not None)
-        if not need:
-            raise TacoError(_lib.last_error())
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ld = self._side(mass, 'mass', torch.float32, B, max_pages * self.page_size)
+        ws, need = self._workspace('taco_kv_attend_workspace_bytes', B, hq, max_pages, mass is not None)
         out = torch.empty((B, hq, self.head_dim), dtype=self.dtype, device=self.device)
         lse = torch.empty((B, hq), dtype=torch.float32, device=self.device)
         self._check(self.lib.taco_kv_attend(
-            self._ref, table.data_ptr(), table.stride(0), B, max_pages, lengths.data_ptr(), q.data_ptr(), q.stride(0),
-            q.stride(1), hq, 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), out.data_ptr(),
+            self._ref, table.data_ptr(), table.stride(0), B, max_pages, lengths.data_ptr(), q.data_ptr(), qs[0],
+            qs[1], hq, 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), out.data_ptr(),
             lse.data_ptr(), mass.data_ptr() if mass is not None else None, ld, ws.data_ptr(), need, self._stream()))
         return out, lse
 
@@ -177,10 +191,10 @@ class KvCache:
         length on get mass 0 and position -1 and their pages may be given away. The pages must belong to one sequence."""
         table = self._table(page_table)
         B, max_pages = table.shape
-        lengths = self._ints(lengths, 'lengths', (B,))
+        lengths = self._ints(lengths, 'lengths', B)
         slots = max_pages * self.page_size
-        ld = self._side(mass, 'mass', torch.float32, B, slots).shape[2]
-        if self._side(positions, 'positions', torch.int32, B, slots).shape[2] != ld:
+        ld = self._side(mass, 'mass', torch.float32, B, slots)
+        if self._side(positions, 'positions', torch.int32, B, slots) != ld:
             raise TacoError('mass and positions must have the same shape')
         budget, recent = int(budget), int(recent)
         if budget < 1 or not 0 <= recent <= budget:
@@ -190,15 +204,12 @@ class KvCache:
             new = (torch.empty_like(lengths), torch.empty_like(mass), torch.empty_like(positions))
         else:
             new = tuple(out)
-            if len(new) != 3 or new[0] is not self._ints(new[0], 'out[0]', (B,)):
+            if len(new) != 3 or new[0] is not self._ints(new[0], 'out[0]', B):
                 raise TacoError('out must be contiguous (lengths, mass, positions) tensors')
-            for name, dtype, t, old in (('out[1]', torch.float32, new[1], mass), ('out[2]', torch.int32, new[2], positions)):
-                if self._side(t, name, dtype, B, slots).shape != old.shape:
+            for name, dtype, t in (('out[1]', torch.float32, new[1]), ('out[2]', torch.int32, new[2])):
+                if self._side(t, name, dtype, B, slots) != ld:
                     raise TacoError('%s must have the shape of its input' % name)
-        need = self.lib.taco_kv_evict_workspace_bytes(self._ref, B, max_pages, budget)
-        if not need:
-            raise TacoError(_lib.last_error())
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        ws, need = self._workspace('taco_kv_evict_workspace_bytes', B, max_pages, budget)
         self._check(self.lib.taco_kv_evict(
             self._ref, table.data_ptr(), table.stride(0), B, max_pages, lengths.data_ptr(), mass.data_ptr(),
             positions.data_ptr(), ld, budget, recent, new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr(),
