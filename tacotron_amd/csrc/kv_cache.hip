@@ -126,9 +126,28 @@ struct AttendShape {
 
 int attend_unit(int dtype) { return dtype == KV_F32 ? AttendShape<KV_F32, 64>::UNIT : AttendShape<KV_BF16, 64>::UNIT; }
 
-__device__ __forceinline__ int wave_sum(int x) {
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+
+// Inclusive sums over the lanes of a wave: within rows of 16 by shifts of 1, 2, 4, 8, then row ends into the rows behind.
+__device__ __forceinline__ int wave_scan(int x) {
+    x = dpp_add<0x111, 0xf>(x);
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);
+    return dpp_add<0x143, 0xc>(x);
+}
+
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
+// f over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48), for each of them.
+template <class F>
+__device__ __forceinline__ float column_all(float x, F f) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // The line of units: sequence b has units(len_b) of them for each of H head groups.
@@ -204,38 +223,42 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
     const int cap = tb.max_pages << p.page_shift, w = blockIdx.x, W = gridDim.x;
     const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
 
-    // sequences without tokens, and the check of the lengths
-    for (int b = w; b < tb.B; b += W)
-        if (clamp_len(a.lengths[b], cap, p.status, tid == 0) == 0) {
-            for (int i = tid; i < hq * D * ES / 4; i += 256) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
-            for (int i = tid; i < hq; i += 256) a.lse[(int64_t)b * hq + i] = -INFINITY;
-        }
-
-    int total = 0;
-    for (int i = lane; i < tb.B; i += 64) total += units_of(tb, a.lengths, i, cap, UNIT);
-    total = __builtin_amdgcn_readfirstlane(wave_sum(total));
+    // the line, from the units of the first 64 sequences (a lane each) and, 64 by 64, the rest
+    const int first64 = lane < tb.B ? units_of(tb, a.lengths, lane, cap, UNIT) : 0;
+    const int scan64 = wave_scan(first64);
+    int total = __builtin_amdgcn_readlane(scan64, 63);
+    if (tb.B > 64) {
+        int more = 0;
+        for (int i = lane + 64; i < tb.B; i += 64) more += units_of(tb, a.lengths, i, cap, UNIT);
+        total += wave_sum(more);
+    }
     const Line line(total * H, W);
     const int u0 = line.begin(w), u1 = line.begin(w + 1);
-    if (u0 == u1) return;
+
+    // sequences without tokens, and the check of the lengths
+    if (u0 == u1 || w < tb.B) {
+        for (int b = w; b < tb.B; b += W)
+            if (clamp_len(a.lengths[b], cap, p.status, tid == 0) == 0) {
+                for (int i = tid; i < hq * D * ES / 4; i += 256) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
+                for (int i = tid; i < hq; i += 256) a.lse[(int64_t)b * hq + i] = -INFINITY;
+            }
+        if (u0 == u1) return;
+    }
+
     int b = 0, before = 0;                           // the sequence of unit u0, and the units before it
-    for (int b0 = 0;; b0 += 64) {
-        const int x = b0 + lane < tb.B ? units_of(tb, a.lengths, b0 + lane, cap, UNIT) * H : 0;
-        int inc = x;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(inc, o);
-            if (lane >= o) inc += y;
-        }
-        const unsigned long long hit = __ballot(before + inc > u0);
+    for (int x = first64, inc = scan64;;) {
+        const unsigned long long hit = __ballot(before + inc * H > u0);
         if (hit) {
             const int at = __ffsll(hit) - 1;
-            b = b0 + at;
-            before += __shfl(inc - x, at);
+            b += at;
+            before += __builtin_amdgcn_readlane(inc - x, at) * H;
             break;
         }
-        before += __shfl(inc, 63);
+        before += __builtin_amdgcn_readlane(inc, 63) * H;
+        b += 64;
+        x = b + lane < tb.B ? units_of(tb, a.lengths, b + lane, cap, UNIT) : 0;
+        inc = wave_scan(x);
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    before = __builtin_amdgcn_readfirstlane(before);
     int nb = units_of(tb, a.lengths, b, cap, UNIT);
     int hg = (u0 - before) / nb, tile = (u0 - before) % nb;
 
@@ -265,11 +288,6 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
         const int64_t kp = p.k_st[0] * ES, kt = p.k_st[2] * ES, vp = p.v_st[0] * ES, vt = p.v_st[2] * ES;
         const int mask = p.page_size - 1;
 
-        u32x4 qf[KL];
-        const char* q = (const char*)a.q + ((int64_t)b * a.q_st[0] + (int64_t)(head0 + col) * a.q_st[1]) * ES + grp * 16;
-#pragma unroll
-        for (int j = 0; j < KL; ++j) qf[j] = col < nh ? *reinterpret_cast<const u32x4*>(q + j * 64) : u32x4{0, 0, 0, 0};
-
         float m = -INFINITY, l = 0.f;
         f32x4 acc[NACC];
 #pragma unroll
@@ -293,6 +311,13 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
         if (t < tend) {
             kpage = page_of(t + ktok);
             vpage = page_of(t + NV * grp);
+        }
+        u32x4 qf[KL];
+        const char* q = (const char*)a.q + ((int64_t)b * a.q_st[0] + (int64_t)(head0 + col) * a.q_st[1]) * ES + grp * 16;
+#pragma unroll
+        for (int j = 0; j < KL; ++j) qf[j] = col < nh ? *reinterpret_cast<const u32x4*>(q + j * 64) : u32x4{0, 0, 0, 0};
+
+        if (t < tend) {
             load_k(t, kpage);
             kpage = page_of(t + UNIT + ktok);
         }
@@ -342,9 +367,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
 #pragma unroll
             for (int i = 1; i < NV; ++i) mx = fmaxf(mx, sc[i]);
             if (__any(mx > m)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float mn = fmaxf(m, mx);
+                const float mn = fmaxf(m, column_all(mx, [](float x, float y) { return fmaxf(x, y); }));
                 const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
                 m = mn;
                 l *= alpha;
@@ -385,8 +408,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const Kv
         }
 
         // the four waves' parts: wave r adds up component r of every accumulator, dims x 16 VEC + (4 grp + r) VEC + e
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
+        l = column_all(l, [](float x, float y) { return x + y; });
         if (grp == 0) ml[wave][col] = float2{m == -INFINITY ? -INFINITY : m - OFF, l};
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -500,8 +522,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         total += n;
         before += i < b ? n : 0;
     }
-    total = __builtin_amdgcn_readfirstlane(wave_sum(total));
-    before = __builtin_amdgcn_readfirstlane(wave_sum(before));
+    total = wave_sum(total);
+    before = wave_sum(before);
     const Line line(total * H, W);
     auto parts_of = [&](int grp16) {
         Parts q;
