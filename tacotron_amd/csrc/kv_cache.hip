@@ -107,8 +107,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int AT_WAVES = 4;
-constexpr int AT_JOIN_MAX = 2048;        // workgroups, at most: parts of a head that kv_join_kernel has room for
-constexpr int MASS_TOKENS = 1024;        // tokens of mass per workgroup
 
 template <int DT, int D>
 struct AttendShape {
@@ -484,33 +482,36 @@ __device__ __forceinline__ float2 stat_join(float2 x, float2 y) {
     return float2{M, x.y * ex2(x.x - ref) + y.y * ex2(y.x - ref)};
 }
 
-// Workgroups 0 .. B * hq - 1: the parts of one (sequence, query head) joined. The rest: MASS_TOKENS tokens of
-// mass[b][h] += sum over the query heads of h of exp(score - lse), from the scores that kv_attend_kernel left. The lse of
-// a head in parts is computed by whoever needs it (a few values), so that both fit one launch. Short work that waits for
-// one dependent load after the other, so every step loads all it needs at once: a part's {exponent, sum} per lane, eight
-// rows of the parts' outputs per lane, four tokens of a head's scores per lane.
-template <int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTable tb, const KvAttend a, int W, int unit) {
-    constexpr int COLS = D / 4, ROWS = 256 / COLS;   // a lane joins four dims of every ROWS-th part
-    __shared__ float fac[AT_JOIN_MAX];
-    __shared__ f32x4 sums[ROWS][COLS];
+// The first `joins` workgroups join the parts of a (sequence, query head): one each, or, WAVES, one per wave. The rest
+// do mass_tokens tokens (a multiple of 1024) of mass[b][h] += sum over the query heads of h of exp(score - lse) each, from
+// the scores that kv_attend_kernel left. The lse of a head in parts is computed by whoever needs it (a few values), so
+// that both fit one launch. Short work that waits for one dependent load after the other, so every step loads all it needs
+// at once: a part's {exponent, sum} per lane, eight rows of the parts' outputs per lane, four tokens of a head's
+// scores per lane.
+template <int D, bool WAVES>
+__global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTable tb, const KvAttend a, int W, int unit, int joins,
+                                                      int mass_tokens) {
+    constexpr int COLS = D / 4;                      // a lane joins four dims of every ROWS-th part
+    constexpr int ROWS = (WAVES ? 64 : 256) / COLS;
+    __shared__ f32x4 sums[WAVES ? 1 : ROWS][WAVES ? 1 : COLS];
     __shared__ float lse2[16];
     __shared__ float2 wave_stat[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cap = tb.max_pages << p.page_shift;
     const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
-    const int joins = tb.B * hq;
     const bool join = (int)blockIdx.x < joins;
     int b, kvh, h0 = 0, t0 = 0;                      // h0: query head within the group
     if (join) {
-        b = blockIdx.x / hq;
-        kvh = blockIdx.x % hq / a.group;
-        h0 = blockIdx.x % hq % a.group;
+        const int i = WAVES ? blockIdx.x * 4 + wave : blockIdx.x;
+        b = i / hq;
+        if (b >= tb.B) return;                       // (no barrier where a wave has its own head)
+        kvh = i % hq / a.group;
+        h0 = i % hq % a.group;
     } else {
-        const int chunks = (cap + MASS_TOKENS - 1) / MASS_TOKENS, i = blockIdx.x - joins;
+        const int chunks = (cap + mass_tokens - 1) / mass_tokens, i = blockIdx.x - joins;
         b = i / (chunks * p.heads);
         kvh = i / chunks % p.heads;
-        t0 = i % chunks * MASS_TOKENS;
+        t0 = i % chunks * mass_tokens;
     }
     const int len = max(0, min(a.lengths[b], cap));
     if (t0 >= len) return;
@@ -543,37 +544,45 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         const Parts q = parts_of(h0 >> 4);
         if (q.w0 == q.w1) return;
         const int c = h0 & 15, n = q.w1 - q.w0 + 1;
-        float2 x = stats(q, c, tid, 256);
-        if (lane == 0) wave_stat[wave] = x;
-        __syncthreads();
-        x = stat_join(stat_join(wave_stat[0], wave_stat[1]), stat_join(wave_stat[2], wave_stat[3]));
+        float2 x = stats(q, c, WAVES ? lane : tid, WAVES ? 64 : 256);
+        if (!WAVES) {
+            if (lane == 0) wave_stat[wave] = x;
+            __syncthreads();
+            x = stat_join(stat_join(wave_stat[0], wave_stat[1]), stat_join(wave_stat[2], wave_stat[3]));
+        }
         const float ref = x.x == -INFINITY ? 0.f : x.x, L = x.y;
-        for (int i = tid; i < n; i += 256) fac[i] = ex2(a.part_ml[q.slot(line, q.w0 + i) * 16 + c].x - ref);
-        __syncthreads();
-        const int d4 = tid % COLS, k = tid / COLS;
+        const int id = WAVES ? lane : tid, d4 = id % COLS, k = id / COLS;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        const float* po = a.part_out + (int64_t)c * D + 4 * d4;
         for (int i = k; i < n; i += 8 * ROWS) {
             f32x4 v[8];
             float f[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int r = min(i + j * ROWS, n - 1);      // (a part beyond the last: the last again, times 0)
-                v[j] = *reinterpret_cast<const f32x4*>(po + (int64_t)q.slot(line, q.w0 + r) * a.score_rows * D);
-                f[j] = fac[r];
+                const int slot = q.slot(line, q.w0 + min(i + j * ROWS, n - 1));      // (beyond the last part: not added)
+                v[j] = *reinterpret_cast<const f32x4*>(a.part_out + ((int64_t)slot * a.score_rows + c) * D + 4 * d4);
+                f[j] = a.part_ml[slot * 16 + c].x;
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (i + j * ROWS < n) o += v[j] * f[j];
+                if (i + j * ROWS < n) o += v[j] * ex2(f[j] - ref);
         }
-        sums[k][d4] = o;
-        __syncthreads();
-        if (k) return;
+        if constexpr (WAVES) {
 #pragma unroll
-        for (int i = 1; i < ROWS; ++i) o += sums[i][d4];
+            for (int step = COLS; step < 64; step *= 2)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], step);
+        } else {
+            sums[k][d4] = o;
+            __syncthreads();
+        }
+        if (k) return;
+        if constexpr (!WAVES) {
+#pragma unroll
+            for (int i = 1; i < ROWS; ++i) o += sums[i][d4];
+        }
         o *= L == 0.f ? 0.f : 1.f / L;
         const int64_t head = (int64_t)b * hq + kvh * a.group + h0;
-        if (tid == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
+        if (id == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int64_t at = head * D + 4 * d4 + e;
@@ -583,11 +592,10 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         }
         return;
     }
-    const int t = t0 + 4 * tid;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    float* mass = a.mass + ((int64_t)b * p.heads + kvh) * a.side_ld;
     for (int g = 0; g < ngrp; ++g) {
         const Parts q = parts_of(g);
-        const int nh = min(16, a.group - 16 * g);
+        const int nh = min(16, a.group - 16 * g), tw = unit / AT_WAVES;
         for (int c = wave; c < nh; c += 4) {
             float x;
             if (q.w0 == q.w1) x = a.lse[(int64_t)b * hq + kvh * a.group + 16 * g + c] * LOG2E;
@@ -599,22 +607,21 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
             if (lane == 0) lse2[c] = x == -INFINITY ? 0.f : x;
         }
         __syncthreads();
-        if (t < len) {                               // (tiles are multiples of 4 tokens: four scores lie together)
-            const int tw = unit / AT_WAVES;
+        for (int t = t0 + 4 * tid; t < min(len, t0 + mass_tokens); t += 1024) {
             const float* s = a.scores + ((int64_t)q.first * AT_WAVES + t / tw) * a.score_rows * tw + t % tw;
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-            for (int c = 0; c < nh; ++c) {
+            for (int c = 0; c < nh; ++c) {           // (tiles are multiples of 4 tokens: four scores lie together)
                 const f32x4 x = *reinterpret_cast<const f32x4*>(s + c * tw);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] += ex2(x[e] - lse2[c]);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (t + e < len) mass[t + e] += sum[e];
         }
         __syncthreads();
     }
-    float* mass = a.mass + ((int64_t)b * p.heads + kvh) * a.side_ld + t;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (t + e < len) mass[e] += sum[e];
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1038,12 +1045,12 @@ bool kv_attend_fits(const KvPool& p, int B, int group, int max_pages) {
     // units are counted in 31 bits on the device, workgroups of 256 threads in 32
     const int64_t cap = (int64_t)max_pages << p.page_shift;
     return attend_units(p, B, group, max_pages) < (1ll << 30) &&
-           (int64_t)B * p.heads * (group + (cap + MASS_TOKENS - 1) / MASS_TOKENS) < (1ll << 24);
+           (int64_t)B * p.heads * (group + (cap + 1023) / 1024) < (1ll << 24);
 }
 
 // Workgroups of the attention: two to a CU keep enough loads in flight, and a unit each where there are fewer units.
 static int attend_shares(const KvPool& p, int B, int group, int max_pages) {
-    return (int)std::min<int64_t>(attend_units(p, B, group, max_pages), std::min(2 * kv_cus(p.device), AT_JOIN_MAX));
+    return (int)std::min<int64_t>(attend_units(p, B, group, max_pages), 2 * kv_cus(p.device));
 }
 
 // {maximum, sum} and output of two parts per workgroup (the one it begins with, the one it ends with), and the scores
@@ -1068,9 +1075,15 @@ static void attend_both(const KvPool& p, const KvTable& tb, const KvAttend& a, i
     const int unit = attend_unit(p.dtype);
     const int64_t cap = (int64_t)tb.max_pages << p.page_shift;
     if (cap <= unit && !a.mass) return;              // nothing is ever in parts
-    int64_t blocks = (int64_t)tb.B * p.heads * a.group;
-    if (a.mass) blocks += (int64_t)tb.B * p.heads * ((cap + MASS_TOKENS - 1) / MASS_TOKENS);
-    kv_join_kernel<D><<<(unsigned)blocks, 256, 0, s>>>(p, tb, a, W, unit);
+    // A wave per head where heads are in few parts, on average; a workgroup where they are in many. Longer stretches of mass
+    // where there are enough of them to fill the chip. (Workgroups of some 4 us each: their number is what counts.)
+    const int64_t heads = (int64_t)tb.B * p.heads * a.group, rows = (int64_t)tb.B * p.heads;
+    const bool waves = W <= 4 * rows * ((a.group + 15) / 16);
+    const int64_t joins = waves ? (heads + 3) / 4 : heads;
+    const int mass_tokens = rows * ((cap + 4095) / 4096) >= 512 ? 4096 : 1024;
+    const int64_t blocks = joins + (a.mass ? rows * ((cap + mass_tokens - 1) / mass_tokens) : 0);
+    if (waves) kv_join_kernel<D, true><<<(unsigned)blocks, 256, 0, s>>>(p, tb, a, W, unit, (int)joins, mass_tokens);
+    else kv_join_kernel<D, false><<<(unsigned)blocks, 256, 0, s>>>(p, tb, a, W, unit, (int)joins, mass_tokens);
 }
 
 void launch_kv_attend(const KvPool& p, const KvTable& tb, KvAttend a, void* ws, hipStream_t s) {
