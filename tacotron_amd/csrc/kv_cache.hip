@@ -82,11 +82,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvPool p, const Kv
 // One pass over the pages with the running maximum and sum of the softmax, on the matrix cores, the token axis cut into
 // equal shares. What bounds it is reading K and V once.
 //
-// Shares. The tokens of a (sequence, kv head) are units of 4 waves x TW tokens; all units of the call, sequence by
-// sequence and head by head, are one line, and workgroup w of W takes the w-th W-th of it. The line is laid out on the
-// device from the lengths, so the split follows the lengths that are there when the kernel (or a captured graph) runs, a
-// ragged batch is as balanced as an even one, and one long sequence fills the chip. Where a head's units end up in several
-// workgroups each leaves {maximum, sum, unnormalised output} in the workspace and kv_join_kernel joins them.
+// Shares. The tokens of a (sequence, kv head) are tiles of TW; all tiles of the call, sequence by sequence and head by head,
+// are one line, and wave w of W takes the w-th W-th of it. The line is laid out on the device from the lengths, so the
+// split follows the lengths that are there when the kernel (or a captured graph) runs, a ragged batch is as balanced as
+// an even one, and one long sequence fills the chip. A wave walks its share tile by tile, from one head into the next, with
+// the next tile's K always in flight, and meets no barrier; four waves to a CU keep enough loads in flight (64 KB), and more
+// of them only spread the reads over more pages at a time. Heads that end up in several waves leave {maximum, sum,
+// unnormalised output} of each in the workspace and kv_join_kernel joins them.
 //
 // Products. Query heads of one kv head are the columns of 16-wide tiles (a group over 16 takes several passes, one under
 // 16 leaves columns idle: the matrix cores have the room, the reads of K and V are what counts).
@@ -111,18 +113,17 @@ constexpr int AT_WAVES = 4;
 template <int DT, int D>
 struct AttendShape {
     static constexpr int ES = DT == KV_F32 ? 4 : 2;
-    static constexpr int TW = DT == KV_F32 ? 16 : 32;          // tokens of a wave's tile
-    static constexpr int UNIT = AT_WAVES * TW;
+    static constexpr int TW = DT == KV_F32 ? 16 : 32;          // tokens of a tile
     static constexpr int VEC = DT != KV_F32 && D >= 128 ? 8 : 4;   // dims per lane and V row
     static constexpr int NX = D / (16 * VEC);
     static constexpr int NACC = D / 16;
     static constexpr int KL = D * ES / 64;                     // 16-byte loads per lane and K row
-    // Floats of scores a wave gathers in LDS: two workgroups' tables fill a CU's 160 KB (one's at D = 256, whose registers
-    // allow no second)
-    static constexpr int GATHER = (D == 64 ? 16 : D == 128 ? 13 : 24) * 256;
 };
 
-int attend_unit(int dtype) { return dtype == KV_F32 ? AttendShape<KV_F32, 64>::UNIT : AttendShape<KV_BF16, 64>::UNIT; }
+// Bytes of scores a wave gathers in LDS: the workgroup's four share the CU's 160 KB.
+constexpr int AT_GATHER = 39 * 1024;
+
+int attend_tile(int dtype) { return dtype == KV_F32 ? AttendShape<KV_F32, 64>::TW : AttendShape<KV_BF16, 64>::TW; }
 
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int dpp_add(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
@@ -148,9 +149,9 @@ __device__ __forceinline__ float column_all(float x, F f) {
     return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// The line of units: sequence b has units(len_b) of them for each of H head groups.
+// The line of tiles: sequence b has tiles(len_b) of them for each of H head groups.
 struct Line {
-    int base, rem;                       // share w: base units, and one more for w < rem
+    int base, rem;                       // share w: base tiles, and one more for w < rem
     __device__ Line(int U, int W) : base(U / W), rem(U % W) {}
     __device__ int begin(int w) const { return w * base + min(w, rem); }
     __device__ int share_of(int u) const {
@@ -159,9 +160,9 @@ struct Line {
     }
 };
 
-__device__ __forceinline__ int units_of(const KvTable& tb, const int32_t* lengths, int b, int cap, int unit) {
+__device__ __forceinline__ int tiles_of(const KvTable& tb, const int32_t* lengths, int b, int cap, int tw) {
     const int n = lengths[b];
-    return n <= 0 ? 0 : (min(n, cap) + unit - 1) / unit;
+    return n <= 0 ? 0 : (min(n, cap) + tw - 1) / tw;
 }
 
 template <int DT>
@@ -202,277 +203,280 @@ __device__ __forceinline__ void split8(const float* p, u32x4* hi, u32x4* lo) {
     *lo = __builtin_bit_cast(u32x4, l);
 }
 
+// A tile of the line.
+struct Cursor {
+    int b, hg, tile;                     // sequence, head group, tile of its tokens
+    int nb, len;                         // tiles and tokens of the sequence
+};
+
 template <int DT, int D, bool MASS>
-__global__ __launch_bounds__(256) void kv_attend_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
+__global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
     using S = AttendShape<DT, D>;
-    constexpr int TW = S::TW, UNIT = S::UNIT, VEC = S::VEC, NX = S::NX, NACC = S::NACC, KL = S::KL, ES = S::ES;
+    constexpr int TW = S::TW, VEC = S::VEC, NX = S::NX, NACC = S::NACC, KL = S::KL, ES = S::ES;
     constexpr int NS = TW / 16, NV = TW / 4;         // 16-token blocks; tokens a lane holds, NV (lane >> 4) and on
     // fp16 weights are kept 2^14 too large (the sums with them): at most 16384, and 2^-28 is still a normal number, so that
     // many small weights beside a large one are not lost
     constexpr float OFF = DT == KV_F16 ? 14.f : 0.f;
     typedef typename std::conditional<VEC * ES == 16, u32x4, u32x2>::type vload_t;
-    __shared__ float xch[4][3][NACC][64];            // quarter, source wave, accumulator, lane
-    __shared__ float2 ml[AT_WAVES][16];
-    __shared__ f32x4 gathered[MASS ? AT_WAVES : 1][MASS ? S::GATHER / 4 : 1];
+    __shared__ f32x4 gathered[MASS ? AT_WAVES : 1][MASS ? AT_GATHER / 16 : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int ktok = NS == 2 ? 8 * (col >> 2) + (col & 3) : col;     // token of this lane's K row, block 0
-    const int cap = tb.max_pages << p.page_shift, w = blockIdx.x, W = gridDim.x;
+    const int cap = tb.max_pages << p.page_shift, w = blockIdx.x * AT_WAVES + wave;
     const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
 
-    // the line, from the units of the first 64 sequences (a lane each) and, 64 by 64, the rest
-    const int first64 = lane < tb.B ? units_of(tb, a.lengths, lane, cap, UNIT) : 0;
+    // the line, from the tiles of the first 64 sequences (a lane each) and, 64 by 64, the rest
+    const int first64 = lane < tb.B ? tiles_of(tb, a.lengths, lane, cap, TW) : 0;
     const int scan64 = wave_scan(first64);
     int total = __builtin_amdgcn_readlane(scan64, 63);
     if (tb.B > 64) {
         int more = 0;
-        for (int i = lane + 64; i < tb.B; i += 64) more += units_of(tb, a.lengths, i, cap, UNIT);
+        for (int i = lane + 64; i < tb.B; i += 64) more += tiles_of(tb, a.lengths, i, cap, TW);
         total += wave_sum(more);
     }
-    const Line line(total * H, W);
+    const Line line(total * H, gridDim.x * AT_WAVES);
     const int u0 = line.begin(w), u1 = line.begin(w + 1);
 
     // sequences without tokens, and the check of the lengths
-    if (u0 == u1 || w < tb.B) {
-        for (int b = w; b < tb.B; b += W)
-            if (clamp_len(a.lengths[b], cap, p.status, tid == 0) == 0) {
-                for (int i = tid; i < hq * D * ES / 4; i += 256) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
-                for (int i = tid; i < hq; i += 256) a.lse[(int64_t)b * hq + i] = -INFINITY;
-            }
-        if (u0 == u1) return;
-    }
+    for (int b = w; b < tb.B; b += gridDim.x * AT_WAVES)
+        if (clamp_len(a.lengths[b], cap, p.status, lane == 0) == 0) {
+            for (int i = lane; i < hq * D * ES / 4; i += 64) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
+            for (int i = lane; i < hq; i += 64) a.lse[(int64_t)b * hq + i] = -INFINITY;
+        }
+    if (u0 == u1) return;
 
-    int b = 0, before = 0;                           // the sequence of unit u0, and the units before it
+    int b0 = 0, before = 0;                          // the sequence of tile u0, and the tiles before it
     for (int x = first64, inc = scan64;;) {
         const unsigned long long hit = __ballot(before + inc * H > u0);
         if (hit) {
             const int at = __ffsll(hit) - 1;
-            b += at;
+            b0 += at;
             before += __builtin_amdgcn_readlane(inc - x, at) * H;
             break;
         }
         before += __builtin_amdgcn_readlane(inc, 63) * H;
-        b += 64;
-        x = b + lane < tb.B ? units_of(tb, a.lengths, b + lane, cap, UNIT) : 0;
+        b0 += 64;
+        x = b0 + lane < tb.B ? tiles_of(tb, a.lengths, b0 + lane, cap, TW) : 0;
         inc = wave_scan(x);
     }
-    int nb = units_of(tb, a.lengths, b, cap, UNIT);
-    int hg = (u0 - before) / nb, tile = (u0 - before) % nb;
+    auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    auto at_sequence = [&](Cursor& c) {
+        c.len = uniform(min(a.lengths[c.b], cap));
+        c.nb = c.len <= 0 ? 0 : (c.len + TW - 1) / TW;
+    };
+    // (called for tiles of the share only, so there is a next one)
+    auto advance = [&](Cursor c) {
+        if (++c.tile == c.nb) {
+            c.tile = 0;
+            if (++c.hg == H) {
+                c.hg = 0;
+                do {
+                    ++c.b;
+                    at_sequence(c);
+                } while (c.nb == 0);
+            }
+        }
+        return c;
+    };
+    Cursor cur;
+    cur.b = uniform(b0);
+    at_sequence(cur);
+    cur.hg = (u0 - before) / cur.nb;
+    cur.tile = (u0 - before) % cur.nb;
 
-    // Scores for the weights of `mass`: [unit][wave][score_rows][TW]. A wave gathers those of its tiles of units gather0,
-    // gather0 + 1, ... and writes them out when there is room for no more, and at the end: a trickle of writes among the
-    // reads costs far more of the memory's time than their bytes.
-    const int tile_vecs = a.score_rows * TW / 4, room = S::GATHER / 4 / tile_vecs;
+    // Page of slot t of a cursor's sequence; of its last one where t lies behind it, so that every row below is in the pool
+    // (and of page 0 where the id is bad): what is masked is read and thrown away. A lane's NV tokens share a page.
+    auto page_of = [&](const Cursor& c, int t) { return tb.table[(int64_t)c.b * tb.ld + (min(c.tile * TW + t, c.len - 1) >> p.page_shift)]; };
+    auto bad_id = [&](int page) { return (unsigned)page >= (unsigned)p.num_pages; };
+    const int mask = p.page_size - 1;
+    u32x4 kf[NS][KL], qf[KL];
+    auto load_k = [&](const Cursor& c, int page) {
+        const int kvh = c.hg / ngrp;
+        const char* r = (const char*)p.k + ((int64_t)kvh * p.k_st[1] + (int64_t)(bad_id(page) ? 0 : page) * p.k_st[0] +
+                                            (int64_t)((c.tile * TW + ktok) & mask) * p.k_st[2]) * ES + grp * 16;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < KL; ++j)
+                kf[s][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(r + 4 * s * p.k_st[2] * ES + j * 64));
+    };
+    auto head0_of = [&](const Cursor& c) { return c.hg / ngrp * a.group + c.hg % ngrp * 16; };
+    auto heads_of = [&](const Cursor& c) { return min(16, a.group - c.hg % ngrp * 16); };
+    auto load_q = [&](const Cursor& c) {
+        const char* q = (const char*)a.q + ((int64_t)c.b * a.q_st[0] + (int64_t)(head0_of(c) + min(col, heads_of(c) - 1)) * a.q_st[1]) * ES + grp * 16;
+#pragma unroll
+        for (int j = 0; j < KL; ++j) qf[j] = *reinterpret_cast<const u32x4*>(q + j * 64);      // (idle columns: the last head again)
+    };
+
+    // Scores for the weights of `mass`: [tile][score_rows][TW]. A wave gathers those of tiles gather0, gather0 + 1, ... and
+    // writes them out when there is room for no more, and at the end: a trickle of writes among the reads costs far more of
+    // the memory's time than their bytes.
+    const int tile_vecs = a.score_rows * TW / 4, room = AT_GATHER / 16 / tile_vecs;
     int gather0 = u0;
     auto flush = [&](int upto) {
-        f32x4* to = (f32x4*)a.scores + ((int64_t)gather0 * AT_WAVES + wave) * tile_vecs;
-        const int n = min(upto - gather0, room);     // (units in which this wave had no tile may lie behind)
+        f32x4* to = (f32x4*)a.scores + (int64_t)gather0 * tile_vecs;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int i = 0; i < n; ++i, to += AT_WAVES * tile_vecs)
-            for (int j = lane; j < tile_vecs; j += 64) to[j] = gathered[wave][i * tile_vecs + j];
+        for (int j = lane; j < (upto - gather0) * tile_vecs; j += 64) to[j] = gathered[wave][j];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         gather0 = upto;
     };
 
-    for (int u = u0; u < u1;) {
-        const int stop = min(nb, tile + (u1 - u));
-        const int len = min(a.lengths[b], cap);
-        const int kvh = hg / ngrp, head0 = kvh * a.group + (hg % ngrp) * 16, nh = min(16, a.group - (hg % ngrp) * 16);
-        const int tend = min(len, stop * UNIT);
-        const int32_t* row = tb.table + (int64_t)b * tb.ld;
-        const char* kbase = (const char*)p.k + (int64_t)kvh * p.k_st[1] * ES;
-        const char* vbase = (const char*)p.v + (int64_t)kvh * p.v_st[1] * ES;
-        const int64_t kp = p.k_st[0] * ES, kt = p.k_st[2] * ES, vp = p.v_st[0] * ES, vt = p.v_st[2] * ES;
-        const int mask = p.page_size - 1;
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc[NACC];
+#pragma unroll
+    for (int n = 0; n < NACC; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int vpage = page_of(cur, NV * grp);
+    load_q(cur);
+    load_k(cur, page_of(cur, ktok));
+    Cursor next = u0 + 1 < u1 ? advance(cur) : cur;
+    int kpage1 = page_of(next, ktok), vpage1 = page_of(next, NV * grp);
+    int seg0 = u0;                                   // where this wave began with the head
 
-        float m = -INFINITY, l = 0.f;
-        f32x4 acc[NACC];
+    for (int u = u0;;) {
+        // pages of the tile after the next, then V of this one: in flight during the first product
+        const bool last = u + 1 == u1;
+        const Cursor next2 = u + 2 < u1 ? advance(next) : next;
+        const int kpage2 = page_of(next2, ktok), vpage2 = page_of(next2, NV * grp);
+        const int t = cur.tile * TW, tok = t + NV * grp;
+        const bool bad = bad_id(vpage);
+        vload_t vf[NV][NX];
+        const char* r = (const char*)p.v + ((int64_t)(cur.hg / ngrp) * p.v_st[1] + (int64_t)(bad ? 0 : vpage) * p.v_st[0] +
+                                            (int64_t)(tok & mask) * p.v_st[2]) * ES + col * VEC * ES;
 #pragma unroll
-        for (int n = 0; n < NACC; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-        // page of slot t; of the share's last one where t lies behind it, so that every row below is in the pool (and
-        // of page 0 where the id is bad): what is masked is read and thrown away. A lane's NV tokens share a page.
-        auto page_of = [&](int t) { return row[min(t, tend - 1) >> p.page_shift]; };
-        auto bad_id = [&](int page) { return (unsigned)page >= (unsigned)p.num_pages; };
-        u32x4 kf[NS][KL];
-        auto load_k = [&](int t, int page) {
-            const char* r = kbase + (int64_t)(bad_id(page) ? 0 : page) * kp + ((t + ktok) & mask) * kt + grp * 16;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
+            for (int x = 0; x < NX; ++x)
+                vf[i][x] = __builtin_nontemporal_load(reinterpret_cast<const vload_t*>(r + i * p.v_st[2] * ES + x * 16 * VEC * ES));
+        float sc[NV];
 #pragma unroll
-                for (int j = 0; j < KL; ++j)
-                    kf[s][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(r + 4 * s * kt + j * 64));
-        };
-        int t = tile * UNIT + wave * TW;
-        int kpage = 0, vpage = 0;
-        if (t < tend) {
-            kpage = page_of(t + ktok);
-            vpage = page_of(t + NV * grp);
+        for (int s = 0; s < NS; ++s) {
+            f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KL; ++j) c = Mma<DT>::run(kf[s][j], qf[j], c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[4 * s + i] = c[i] * a.scale2;
         }
-        u32x4 qf[KL];
-        const char* q = (const char*)a.q + ((int64_t)b * a.q_st[0] + (int64_t)(head0 + col) * a.q_st[1]) * ES + grp * 16;
-#pragma unroll
-        for (int j = 0; j < KL; ++j) qf[j] = col < nh ? *reinterpret_cast<const u32x4*>(q + j * 64) : u32x4{0, 0, 0, 0};
-
-        if (t < tend) {
-            load_k(t, kpage);
-            kpage = page_of(t + UNIT + ktok);
+        const bool end = last || next.tile == 0;     // of the head, as far as it is this wave's
+        const int nh = heads_of(cur);
+        if (!last) {
+            if (end) load_q(next);
+            load_k(next, kpage1);
         }
-        for (; t < tend; t += UNIT) {
-            // pages of the tile after the next, then V of this one: in flight during the first product
-            const int kpage2 = page_of(t + 2 * UNIT + ktok), vpage2 = page_of(t + UNIT + NV * grp);
-            const int tok = t + NV * grp;
-            const bool bad = bad_id(vpage);
-            vload_t vf[NV][NX];
-            const char* r = vbase + (int64_t)(bad ? 0 : vpage) * vp + (tok & mask) * vt + col * VEC * ES;
+        if (t + TW > cur.len || __any(bad)) {
+            // masked slots: score -inf, and no row that 0 could be multiplied with to give NaN
+            if (bad && tok < cur.len) atomicOr(p.status, KV_BAD_PAGE);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
+                if (bad || tok + i >= cur.len) {
+                    sc[i] = -INFINITY;
+#pragma unroll
+                    for (int x = 0; x < NX; ++x) vf[i][x] = vload_t{};
+                }
+        }
+        if constexpr (MASS) {
+            if (u - gather0 == room) flush(u);
+            if (col < nh) {
+                f32x4* to = gathered[wave] + (u - gather0) * tile_vecs + (col * TW + NV * grp) / 4;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) to[s] = f32x4{sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]};
+            }
+        }
+        float mx = sc[0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) mx = fmaxf(mx, sc[i]);
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, column_all(mx, [](float x, float y) { return fmaxf(x, y); }));
+            const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int n = 0; n < NACC; ++n) acc[n] *= alpha;
+        }
+        const float ref = m == -INFINITY ? 0.f : m - OFF;
+        float pr[NV], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) { pr[i] = ex2(sc[i] - ref); sum += pr[i]; }
+        l += sum;
+        if constexpr (DT == KV_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int x = 0; x < NX; ++x)
-                    vf[i][x] = __builtin_nontemporal_load(reinterpret_cast<const vload_t*>(r + i * vt + x * 16 * VEC * ES));
-            float sc[NV];
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+                    for (int e = 0; e < 4; ++e)
+                        acc[4 * x + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][x][e]), pr[i], acc[4 * x + e], 0, 0, 0);
+        } else {
+            u32x4 hi, lo;
+            if constexpr (DT == KV_BF16) split8<bf16x8>(pr, &hi, &lo);
+            else split8<f16x8>(pr, &hi, &lo);
 #pragma unroll
-                for (int j = 0; j < KL; ++j) c = Mma<DT>::run(kf[s][j], qf[j], c);
+            for (int x = 0; x < NX; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[4 * s + i] = c[i] * a.scale2;
-            }
-            if (t + UNIT < tend) load_k(t + UNIT, kpage);
-            if (t + TW > tend || __any(bad)) {
-                // masked slots: score -inf, and no row that 0 could be multiplied with to give NaN
-                if (bad && tok < tend) atomicOr(p.status, KV_BAD_PAGE);
+                for (int e = 0; e < VEC; ++e) {
+                    u32x4 v;
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (bad || tok + i >= tend) {
-                        sc[i] = -INFINITY;
-#pragma unroll
-                        for (int x = 0; x < NX; ++x) vf[i][x] = vload_t{};
-                    }
-            }
-            if constexpr (MASS) {
-                const int unit = u - tile + t / UNIT;
-                if (unit - gather0 >= room) flush(unit);
-                if (col < nh) {
-                    f32x4* to = gathered[wave] + (unit - gather0) * tile_vecs + (col * TW + NV * grp) / 4;
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) to[s] = f32x4{sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]};
+                    for (int i = 0; i < 4; ++i)
+                        v[i] = __builtin_amdgcn_perm(vf[2 * i + 1][x][e >> 1], vf[2 * i][x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                    acc[x * VEC + e] = Mma<DT>::run(v, hi, acc[x * VEC + e]);
+                    acc[x * VEC + e] = Mma<DT>::run(v, lo, acc[x * VEC + e]);
                 }
-            }
-            float mx = sc[0];
-#pragma unroll
-            for (int i = 1; i < NV; ++i) mx = fmaxf(mx, sc[i]);
-            if (__any(mx > m)) {
-                const float mn = fmaxf(m, column_all(mx, [](float x, float y) { return fmaxf(x, y); }));
-                const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
-                m = mn;
-                l *= alpha;
-#pragma unroll
-                for (int n = 0; n < NACC; ++n) acc[n] *= alpha;
-            }
-            const float ref = m == -INFINITY ? 0.f : m - OFF;
-            float pr[NV], sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) { pr[i] = ex2(sc[i] - ref); sum += pr[i]; }
-            l += sum;
-            if constexpr (DT == KV_F32) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
+        }
+        if (end) {
+            // component i of accumulator x VEC + e is dim 16 VEC x + (4 grp + i) VEC + e of head col
+            const float L = column_all(l, [](float x, float y) { return x + y; });
+            if (col < nh) {
+                const bool whole = seg0 + cur.nb == u + 1;
+                const int d0 = 4 * grp * VEC;
+                if (whole) {
+                    // no weight at all (every page bad, or every score -inf): as a row without tokens
+                    const float inv = L == 0.f ? 0.f : 1.f / L;
+                    const int64_t head = (int64_t)cur.b * hq + head0_of(cur) + col;
+                    if (grp == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
 #pragma unroll
                     for (int x = 0; x < NX; ++x)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            acc[4 * x + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][x][e]), pr[i], acc[4 * x + e], 0, 0, 0);
-            } else {
-                u32x4 hi, lo;
-                if constexpr (DT == KV_BF16) split8<bf16x8>(pr, &hi, &lo);
-                else split8<f16x8>(pr, &hi, &lo);
+                        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int x = 0; x < NX; ++x)
+                            for (int e = 0; e < VEC; ++e) {
+                                const int64_t at = head * D + x * 16 * VEC + d0 + i * VEC + e;
+                                const float o = acc[x * VEC + e][i] * inv;
+                                if constexpr (DT == KV_F32) ((float*)a.out)[at] = o;
+                                else if constexpr (DT == KV_BF16) ((bf16_t*)a.out)[at] = (bf16_t)o;
+                                else ((f16_t*)a.out)[at] = (f16_t)o;
+                            }
+                } else {
+                    const int slot = 2 * w + (seg0 != u0);
+                    if (grp == 0) a.part_ml[slot * 16 + col] = float2{m == -INFINITY ? -INFINITY : ref, L};
+                    float* po = a.part_out + ((int64_t)slot * a.score_rows + col) * D + d0;
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        u32x4 v;
+                    for (int x = 0; x < NX; ++x)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            v[i] = __builtin_amdgcn_perm(vf[2 * i + 1][x][e >> 1], vf[2 * i][x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-                        acc[x * VEC + e] = Mma<DT>::run(v, hi, acc[x * VEC + e]);
-                        acc[x * VEC + e] = Mma<DT>::run(v, lo, acc[x * VEC + e]);
-                    }
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) po[x * 16 * VEC + i * VEC + e] = acc[x * VEC + e][i];
+                }
             }
-            kpage = kpage2;
-            vpage = vpage2;
+            if (last) break;
+            seg0 = u + 1;
+            m = -INFINITY;
+            l = 0.f;
+#pragma unroll
+            for (int n = 0; n < NACC; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-
-        // the four waves' parts: wave r adds up component r of every accumulator, dims x 16 VEC + (4 grp + r) VEC + e
-        l = column_all(l, [](float x, float y) { return x + y; });
-        if (grp == 0) ml[wave][col] = float2{m == -INFINITY ? -INFINITY : m - OFF, l};
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (r != wave) {
-#pragma unroll
-                for (int n = 0; n < NACC; ++n) xch[r][wave - (wave > r)][n][lane] = acc[n][r];
-            }
-        __syncthreads();
-        float M = -INFINITY, L = 0.f, fac[AT_WAVES];
-#pragma unroll
-        for (int i = 0; i < AT_WAVES; ++i) M = fmaxf(M, ml[i][col].x);
-        const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll
-        for (int i = 0; i < AT_WAVES; ++i) { fac[i] = ex2(ml[i][col].x - ref); L += fac[i] * ml[i][col].y; }
-        float o[NACC];
-#pragma unroll
-        for (int n = 0; n < NACC; ++n) {
-            o[n] = (wave == 0 ? acc[n][0] : wave == 1 ? acc[n][1] : wave == 2 ? acc[n][2] : acc[n][3]) * fac[wave];
-#pragma unroll
-            for (int i = 0; i < AT_WAVES; ++i)
-                if (i != wave) o[n] += xch[wave][i - (i > wave)][n][lane] * fac[i];
-        }
-        if (col < nh) {
-            const int d0 = (4 * grp + wave) * VEC;
-            const bool whole = tile == 0 && stop == nb;
-            if (whole) {
-                // no weight at all (every page bad, or every score -inf): as a row without tokens
-                const float inv = L == 0.f ? 0.f : 1.f / L;
-                const int64_t head = (int64_t)b * hq + head0 + col;
-                if (wave == 0 && grp == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
-#pragma unroll
-                for (int x = 0; x < NX; ++x)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const int64_t at = head * D + x * 16 * VEC + d0 + e;
-                        if constexpr (DT == KV_F32) ((float*)a.out)[at] = o[x * VEC + e] * inv;
-                        else if constexpr (DT == KV_BF16) ((bf16_t*)a.out)[at] = (bf16_t)(o[x * VEC + e] * inv);
-                        else ((f16_t*)a.out)[at] = (f16_t)(o[x * VEC + e] * inv);
-                    }
-            } else {
-                const int slot = 2 * w + (u != u0);
-                if (wave == 0 && grp == 0) a.part_ml[slot * 16 + col] = float2{M, L};
-                float* po = a.part_out + ((int64_t)slot * a.score_rows + col) * D + d0;
-#pragma unroll
-                for (int x = 0; x < NX; ++x)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) po[x * 16 * VEC + e] = o[x * VEC + e];
-            }
-        }
-        u += stop - tile;
-        tile = 0;
-        if (u < u1) {
-            __syncthreads();                         // the exchange is read before the next part writes it
-            if (++hg == H) {
-                hg = 0;
-                do nb = units_of(tb, a.lengths, ++b, cap, UNIT);
-                while (nb == 0);
-            }
-        }
+        ++u;
+        cur = next;
+        next = next2;
+        vpage = vpage1;
+        kpage1 = kpage2;
+        vpage1 = vpage2;
     }
     if constexpr (MASS) flush(u1);
 }
 
-// Parts of one (sequence, head group): workgroups w0 .. w1, and where part w of them lies in the workspace.
+// Parts of one (sequence, head group): waves w0 .. w1, and where part w of them lies in the workspace.
 struct Parts {
-    int first, w0, w1;                   // first unit
+    int first, w0, w1;                   // first tile
     __device__ int slot(const Line& line, int w) const { return 2 * w + (line.begin(w) < first); }
 };
 
@@ -489,7 +493,7 @@ __device__ __forceinline__ float2 stat_join(float2 x, float2 y) {
 // at once: a part's {exponent, sum} per lane, eight rows of the parts' outputs per lane, four tokens of a head's
 // scores per lane.
 template <int D, bool WAVES>
-__global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTable tb, const KvAttend a, int W, int unit, int joins,
+__global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTable tb, const KvAttend a, int W, int tw, int joins,
                                                       int mass_tokens) {
     constexpr int COLS = D / 4;                      // a lane joins four dims of every ROWS-th part
     constexpr int ROWS = (WAVES ? 64 : 256) / COLS;
@@ -515,11 +519,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
     }
     const int len = max(0, min(a.lengths[b], cap));
     if (t0 >= len) return;
-    const int nb = (len + unit - 1) / unit;
-    if (join && nb == 1) return;                     // a single unit is never in parts
+    const int nb = (len + tw - 1) / tw;
+    if (join && nb == 1) return;                     // a single tile is never in parts
     int total = 0, before = 0;
     for (int i = lane; i < tb.B; i += 64) {
-        const int n = units_of(tb, a.lengths, i, cap, unit);
+        const int n = tiles_of(tb, a.lengths, i, cap, tw);
         total += n;
         before += i < b ? n : 0;
     }
@@ -595,7 +599,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
     float* mass = a.mass + ((int64_t)b * p.heads + kvh) * a.side_ld;
     for (int g = 0; g < ngrp; ++g) {
         const Parts q = parts_of(g);
-        const int nh = min(16, a.group - 16 * g), tw = unit / AT_WAVES;
+        const int nh = min(16, a.group - 16 * g);
         for (int c = wave; c < nh; c += 4) {
             float x;
             if (q.w0 == q.w1) x = a.lse[(int64_t)b * hq + kvh * a.group + 16 * g + c] * LOG2E;
@@ -608,7 +612,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         }
         __syncthreads();
         for (int t = t0 + 4 * tid; t < min(len, t0 + mass_tokens); t += 1024) {
-            const float* s = a.scores + ((int64_t)q.first * AT_WAVES + t / tw) * a.score_rows * tw + t % tw;
+            const float* s = a.scores + (int64_t)(q.first + t / tw) * a.score_rows * tw + t % tw;
             f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
             for (int c = 0; c < nh; ++c) {           // (tiles are multiples of 4 tokens: four scores lie together)
@@ -1035,36 +1039,36 @@ void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hip
     kv_append_kernel<<<dim3((unsigned)((copies + 255) / 256), tb.B, side ? 3 : 2), 256, 0, s>>>(p, tb, a);
 }
 
-// Units of the line if every sequence filled its table.
-static int64_t attend_units(const KvPool& p, int B, int group, int max_pages) {
-    const int unit = attend_unit(p.dtype);
-    return (((int64_t)max_pages << p.page_shift) + unit - 1) / unit * B * p.heads * ((group + 15) / 16);
+// Tiles of the line if every sequence filled its table.
+static int64_t attend_tiles(const KvPool& p, int B, int group, int max_pages) {
+    const int tw = attend_tile(p.dtype);
+    return (((int64_t)max_pages << p.page_shift) + tw - 1) / tw * B * p.heads * ((group + 15) / 16);
 }
 
 bool kv_attend_fits(const KvPool& p, int B, int group, int max_pages) {
-    // units are counted in 31 bits on the device, workgroups of 256 threads in 32
+    // tiles are counted in 31 bits on the device, workgroups of 256 threads in 32
     const int64_t cap = (int64_t)max_pages << p.page_shift;
-    return attend_units(p, B, group, max_pages) < (1ll << 30) &&
+    return attend_tiles(p, B, group, max_pages) < (1ll << 30) &&
            (int64_t)B * p.heads * (group + (cap + 1023) / 1024) < (1ll << 24);
 }
 
-// Workgroups of the attention: two to a CU keep enough loads in flight, and a unit each where there are fewer units.
-static int attend_shares(const KvPool& p, int B, int group, int max_pages) {
-    return (int)std::min<int64_t>(attend_units(p, B, group, max_pages), 2 * kv_cus(p.device));
+// Workgroups of the attention: one to a CU, or a tile for every wave where there are fewer.
+static int attend_groups(const KvPool& p, int B, int group, int max_pages) {
+    return (int)std::min<int64_t>((attend_tiles(p, B, group, max_pages) + AT_WAVES - 1) / AT_WAVES, kv_cus(p.device));
 }
 
-// {maximum, sum} and output of two parts per workgroup (the one it begins with, the one it ends with), and the scores
+// {maximum, sum} and output of two parts per wave (the one it begins with, the one it ends with), and the scores
 size_t kv_attend_ws_bytes(const KvPool& p, int B, int group, int max_pages, bool mass) {
-    const size_t parts = 2 * (size_t)attend_shares(p, B, group, max_pages), rows = (size_t)std::min(group, 16);
+    const size_t parts = 2 * AT_WAVES * (size_t)attend_groups(p, B, group, max_pages), rows = (size_t)std::min(group, 16);
     size_t n = parts * 16 * sizeof(float2) + parts * rows * p.dim * sizeof(float);
-    if (mass) n += (size_t)attend_units(p, B, group, max_pages) * rows * attend_unit(p.dtype) * sizeof(float);
+    if (mass) n += (size_t)attend_tiles(p, B, group, max_pages) * rows * attend_tile(p.dtype) * sizeof(float);
     return n;
 }
 
 template <int DT, int D>
 static void attend_launch(const KvPool& p, const KvTable& tb, const KvAttend& a, int W, hipStream_t s) {
-    if (a.mass) kv_attend_kernel<DT, D, true><<<W, 256, 0, s>>>(p, tb, a);
-    else kv_attend_kernel<DT, D, false><<<W, 256, 0, s>>>(p, tb, a);
+    if (a.mass) kv_attend_kernel<DT, D, true><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
+    else kv_attend_kernel<DT, D, false><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
 }
 
 template <int D>
@@ -1072,26 +1076,26 @@ static void attend_both(const KvPool& p, const KvTable& tb, const KvAttend& a, i
     if (p.dtype == KV_F32) attend_launch<KV_F32, D>(p, tb, a, W, s);
     else if (p.dtype == KV_BF16) attend_launch<KV_BF16, D>(p, tb, a, W, s);
     else attend_launch<KV_F16, D>(p, tb, a, W, s);
-    const int unit = attend_unit(p.dtype);
+    const int tw = attend_tile(p.dtype), waves_all = W * AT_WAVES;
     const int64_t cap = (int64_t)tb.max_pages << p.page_shift;
-    if (cap <= unit && !a.mass) return;              // nothing is ever in parts
+    if (cap <= tw && !a.mass) return;                // nothing is ever in parts
     // A wave per head where heads are in few parts, on average; a workgroup where they are in many. Longer stretches of mass
     // where there are enough of them to fill the chip. (Workgroups of some 4 us each: their number is what counts.)
     const int64_t heads = (int64_t)tb.B * p.heads * a.group, rows = (int64_t)tb.B * p.heads;
-    const bool waves = W <= 4 * rows * ((a.group + 15) / 16);
+    const bool waves = waves_all <= 8 * rows * ((a.group + 15) / 16);
     const int64_t joins = waves ? (heads + 3) / 4 : heads;
     const int mass_tokens = rows * ((cap + 4095) / 4096) >= 512 ? 4096 : 1024;
     const int64_t blocks = joins + (a.mass ? rows * ((cap + mass_tokens - 1) / mass_tokens) : 0);
-    if (waves) kv_join_kernel<D, true><<<(unsigned)blocks, 256, 0, s>>>(p, tb, a, W, unit, (int)joins, mass_tokens);
-    else kv_join_kernel<D, false><<<(unsigned)blocks, 256, 0, s>>>(p, tb, a, W, unit, (int)joins, mass_tokens);
+    if (waves) kv_join_kernel<D, true><<<(unsigned)blocks, 256, 0, s>>>(p, tb, a, waves_all, tw, (int)joins, mass_tokens);
+    else kv_join_kernel<D, false><<<(unsigned)blocks, 256, 0, s>>>(p, tb, a, waves_all, tw, (int)joins, mass_tokens);
 }
 
 void launch_kv_attend(const KvPool& p, const KvTable& tb, KvAttend a, void* ws, hipStream_t s) {
-    const int W = attend_shares(p, tb.B, a.group, tb.max_pages);
+    const int W = attend_groups(p, tb.B, a.group, tb.max_pages), parts = 2 * W * AT_WAVES;
     a.score_rows = std::min(a.group, 16);
     a.part_ml = (float2*)ws;
-    a.part_out = (float*)(a.part_ml + (size_t)2 * W * 16);
-    a.scores = a.part_out + (size_t)2 * W * a.score_rows * p.dim;
+    a.part_out = (float*)(a.part_ml + (size_t)parts * 16);
+    a.scores = a.part_out + (size_t)parts * a.score_rows * p.dim;
     if (p.dim == 64) attend_both<64>(p, tb, a, W, s);
     else if (p.dim == 128) attend_both<128>(p, tb, a, W, s);
     else attend_both<256>(p, tb, a, W, s);
