@@ -226,9 +226,11 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
     const int cap = tb.max_pages << p.page_shift, w = blockIdx.x * AT_WAVES + wave;
     const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
 
-    // the line, from the tiles of the first 64 sequences (a lane each) and, 64 by 64, the rest
-    const int first64 = lane < tb.B ? tiles_of(tb, a.lengths, lane, cap, TW) : 0;
-    const int scan64 = wave_scan(first64);
+    // the line, from the tiles of the first 64 sequences (a lane each; their lengths stay at hand) and, 64 by 64, the rest
+    auto tiles = [](int len) { return (len + TW - 1) / TW; };
+    const int raw64 = lane < tb.B ? a.lengths[lane] : 0, len64 = max(0, min(raw64, cap));
+    auto len_of = [&](int b) { return b < 64 ? __builtin_amdgcn_readlane(len64, b) : __builtin_amdgcn_readfirstlane(max(0, min(a.lengths[b], cap))); };
+    const int first64 = tiles(len64), scan64 = wave_scan(first64);
     int total = __builtin_amdgcn_readlane(scan64, 63);
     if (tb.B > 64) {
         int more = 0;
@@ -238,12 +240,14 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
     const Line line(total * H, gridDim.x * AT_WAVES);
     const int u0 = line.begin(w), u1 = line.begin(w + 1);
 
-    // sequences without tokens, and the check of the lengths
-    for (int b = w; b < tb.B; b += gridDim.x * AT_WAVES)
-        if (clamp_len(a.lengths[b], cap, p.status, lane == 0) == 0) {
-            for (int i = lane; i < hq * D * ES / 4; i += 64) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
-            for (int i = lane; i < hq; i += 64) a.lse[(int64_t)b * hq + i] = -INFINITY;
-        }
+    // the check of the lengths, and sequences without tokens
+    if (w == 0 && len64 != raw64) atomicOr(p.status, KV_BAD_LENGTH);
+    for (int b = w; b < tb.B; b += gridDim.x * AT_WAVES) {
+        if (b >= 64) (void)clamp_len(a.lengths[b], cap, p.status, lane == 0);
+        if (len_of(b)) continue;
+        for (int i = lane; i < hq * D * ES / 4; i += 64) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
+        for (int i = lane; i < hq; i += 64) a.lse[(int64_t)b * hq + i] = -INFINITY;
+    }
     if (u0 == u1) return;
 
     int b0 = 0, before = 0;                          // the sequence of tile u0, and the tiles before it
@@ -260,10 +264,9 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
         x = b0 + lane < tb.B ? tiles_of(tb, a.lengths, b0 + lane, cap, TW) : 0;
         inc = wave_scan(x);
     }
-    auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     auto at_sequence = [&](Cursor& c) {
-        c.len = uniform(min(a.lengths[c.b], cap));
-        c.nb = c.len <= 0 ? 0 : (c.len + TW - 1) / TW;
+        c.len = len_of(c.b);
+        c.nb = tiles(c.len);
     };
     // (called for tiles of the share only, so there is a next one)
     auto advance = [&](Cursor c) {
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
         return c;
     };
     Cursor cur;
-    cur.b = uniform(b0);
+    cur.b = __builtin_amdgcn_readfirstlane(b0);
     at_sequence(cur);
     cur.hg = (u0 - before) / cur.nb;
     cur.tile = (u0 - before) % cur.nb;
