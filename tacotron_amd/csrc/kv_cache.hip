@@ -17,6 +17,9 @@ namespace {
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
+// a lambda that is not inlined would keep the registers it refers to in memory
+#define INLINE __attribute__((always_inline))
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }   // (flushes results below 2^-126)
@@ -152,9 +155,9 @@ __device__ __forceinline__ float column_all(float x, F f) {
 // The line of tiles: sequence b has tiles(len_b) of them for each of H head groups.
 struct Line {
     int base, rem;                       // share w: base tiles, and one more for w < rem
-    __device__ Line(int U, int W) : base(U / W), rem(U % W) {}
-    __device__ int begin(int w) const { return w * base + min(w, rem); }
-    __device__ int share_of(int u) const {
+    __device__ __forceinline__ Line(int U, int W) : base(U / W), rem(U % W) {}
+    __device__ __forceinline__ int begin(int w) const { return w * base + min(w, rem); }
+    __device__ __forceinline__ int share_of(int u) const {
         const int big = rem * (base + 1);
         return u < big ? u / (base + 1) : rem + (u - big) / base;
     }
@@ -480,7 +483,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
 // Parts of one (sequence, head group): waves w0 .. w1, and where part w of them lies in the workspace.
 struct Parts {
     int first, w0, w1;                   // first tile
-    __device__ int slot(const Line& line, int w) const { return 2 * w + (line.begin(w) < first); }
+    __device__ __forceinline__ int slot(const Line& line, int w) const { return 2 * w + (line.begin(w) < first); }
 };
 
 // {reference exponent, sum} of two disjoint sets of weights as one.
@@ -660,9 +663,8 @@ struct Head {
     const float* mass; const int32_t* pos;
     float* mass_out; int32_t* pos_out;
     int32_t* gaps; int32_t* late; int32_t* counts;
-    int64_t border;                                  // positions above it are protected
-    bool recent;
-    __device__ Head(const KvPool& p, const KvTable& tb, const KvEvict& a, int h, int b, bool report) {
+    int border;                                      // positions above it are protected
+    __device__ __forceinline__ Head(const KvPool& p, const KvTable& tb, const KvEvict& a, int h, int b, bool report) {
         len = clamp_len(a.lengths[b], tb.max_pages << p.page_shift, p.status, report);
         n = min(len, a.budget);
         const int64_t row = (int64_t)b * p.heads + h;
@@ -673,30 +675,60 @@ struct Head {
         gaps = a.lists + row * 2 * a.list_ld;
         late = gaps + a.list_ld;
         counts = a.counts + 2 * row;
-        recent = a.recent > 0;
-        border = INT64_MAX;
+        border = 0x7fffffff;
     }
-    // the key of slot s, 0 from stop on
-    __device__ __forceinline__ uint32_t key(int s, int stop) const {
-        const int t = min(s, stop - 1);
-        uint32_t k = mass_key(mass[t]);
-        if (recent && (int64_t)pos[t] > border) k = 0xffffffffu;
-        return s < stop ? k : 0u;
+    __device__ __forceinline__ void protect(int newest, int recent) {
+        if (recent > 0) border = (int)max((int64_t)newest - recent, (int64_t)(-0x7fffffff - 1));
     }
 };
 
-// f(i) for rows i < per of a wave, i a constant, in groups of up to 8 (rows behind per up to a group's end too).
-template <int R, class F>
+// f(i) for rows i < per of a wave, in groups of 4 (rows behind per up to a group's end too). i is a compile-time constant, as
+// an index into registers has to be.
+template <int R, int I = 0, class F>
 __device__ __forceinline__ void for_rows(int per, F f) {
-    constexpr int G = R < 8 ? R : 8;
-#pragma unroll
-    for (int g = 0; g < R; g += G)
-        if (g < per) {
-#pragma unroll
-            for (int j = 0; j < G; ++j) f(g + j);
+    if constexpr (I < R) {
+        if (I < per) {
+            f(std::integral_constant<int, I>{});
+            f(std::integral_constant<int, I + 1>{});
+            f(std::integral_constant<int, I + 2>{});
+            f(std::integral_constant<int, I + 3>{});
             __builtin_amdgcn_sched_barrier(0);       // keeps one group's masks from living through all of them
+            for_rows<R, I + 4>(per, f);
         }
+    }
 }
+
+// A lane's slots of a head: rows of 64 slots, first + 64 i. Masses and positions come in once; keys are made of them.
+template <int R>
+struct Slots {
+    float mass[R];
+    int pos[R];
+    int first, stop;                                 // slots from stop on are none
+    // (rows behind per, and slots behind stop, read the last slot; the wave has slots, or nothing is read)
+    __device__ __forceinline__ void load(const Head& h, int first_, int stop_, int per) {
+        first = first_;
+        stop = stop_;
+        if (first - (int)(threadIdx.x & 63) >= stop) return;
+        for_rows<R>(per, [&](auto i) INLINE {
+            const int t = min(first + 64 * i, stop - 1);
+            mass[i] = h.mass[t];
+            pos[i] = h.pos[t];
+        });
+    }
+    __device__ __forceinline__ int slot(int i) const { return first + 64 * i; }
+    __device__ __forceinline__ int newest(int per) const {
+        int x = -0x7fffffff - 1;
+        for_rows<R>(per, [&](auto i) INLINE {
+            if (i < per && slot(i) < stop) x = max(x, pos[i]);
+        });
+        return x;
+    }
+    // 0 for no slot
+    __device__ __forceinline__ uint32_t key(const Head& h, int i, int per) const {
+        const uint32_t k = pos[i] > h.border ? 0xffffffffu : mass_key(mass[i]);
+        return i < per && slot(i) < stop ? k : 0u;
+    }
+};
 
 // Counts a key's digit if `in`. Equal digits side by side (fresh tokens, protected ones) would queue for one counter: where
 // a wave has only one digit it adds once.
@@ -758,7 +790,7 @@ __device__ __forceinline__ void pick_rest(SelectShared& sh, E each, uint32_t* th
     for (int pass = 0; pass < 2; ++pass) {
         const int shift = pass ? 0 : 10, bits = pass ? 10 : 11;
         const uint32_t t = *thr;
-        each([&](uint32_t k) { count_digit(sh, k != 0u && k >> (shift + bits) == t >> (shift + bits), k >> shift & ((1u << bits) - 1)); });
+        each([&](uint32_t k) INLINE { count_digit(sh, k != 0u && k >> (shift + bits) == t >> (shift + bits), k >> shift & ((1u << bits) - 1)); });
         __syncthreads();
         pick_digit(sh, *need);
         *thr |= sh.digit << shift;
@@ -770,28 +802,26 @@ __device__ __forceinline__ void pick_rest(SelectShared& sh, E each, uint32_t* th
     }
 }
 
-// Greatest position of slots from .. stop - 1 step 64 over the workgroup into sh.newest (set to the least before).
-__device__ __forceinline__ void newest_of(SelectShared& sh, const int32_t* pos, int from, int stop) {
-    int x = -0x7fffffff - 1;
-#pragma unroll 8
-    for (int s = from; s < stop; s += 64) x = max(x, pos[s]);
+// Greatest of x over the workgroup, in sh.newest (set to the least before). Ends with a barrier.
+__device__ __forceinline__ int block_max(SelectShared& sh, int x) {
     for (int o = 32; o; o >>= 1) x = max(x, __shfl_xor(x, o));
     if ((threadIdx.x & 63) == 0) atomicMax(&sh.newest, x);
     __syncthreads();
+    return sh.newest;
 }
 
-// The outcome for a workgroup's slots: waves one after the other, `per` rows of 64 each from slot0 on, below stop. gt, eq:
-// keys above the threshold and at it in the slots before slot0. All above it are kept and the first `need` at it. A gap
-// below n is the (slot - kept before it)-th, a kept slot from n on has rank `kept before it`: both lists come out
-// ascending without a sort.
+// The outcome for a workgroup's slots: waves one after the other, `per` rows of 64 each. gt, eq: keys above the threshold
+// and at it in the slots before the workgroup's. All above it are kept and the first `need` at it. A gap below n is the
+// (slot - kept before it)-th, a kept slot from n on has rank `kept before it`: both lists come out ascending without a
+// sort.
 template <int R>
-__device__ __forceinline__ void emit(SelectShared& sh, const Head& a, const uint32_t* keys, int slot0, int per, int stop, uint32_t thr,
-                                     int need, int gt, int eq) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ void emit(SelectShared& sh, const Head& a, const Slots<R>& x, int per, uint32_t thr, int need, int gt, int eq) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int g = 0, e0 = 0;
-    for_rows<R>(per, [&](int i) {
-        g += __popcll(__ballot(keys[i] > thr));
-        e0 += __popcll(__ballot(keys[i] == thr));
+    for_rows<R>(per, [&](auto i) INLINE {
+        const uint32_t k = x.key(a, i, per);
+        g += __popcll(__ballot(k > thr));
+        e0 += __popcll(__ballot(k == thr));
     });
     if (lane == 0) { sh.wave_a[wave] = g; sh.wave_b[wave] = e0; }
     __syncthreads();
@@ -801,9 +831,9 @@ __device__ __forceinline__ void emit(SelectShared& sh, const Head& a, const uint
     }
     const unsigned long long low = (1ull << lane) - 1;
     const bool copy = a.mass_out != a.mass, copy_pos = a.pos_out != a.pos;
-    for_rows<R>(per, [&](int i) {
-        const int s = slot0 + (wave * per + i) * 64 + lane;
-        const uint32_t k = keys[i];
+    for_rows<R>(per, [&](auto i) INLINE {
+        const int s = x.slot(i);
+        const uint32_t k = x.key(a, i, per);
         const unsigned long long bg = __ballot(k > thr), be = __ballot(k == thr);
         const int e = eq + __popcll(be & low), before = gt + __popcll(bg & low) + min(e, need);
         const bool keep = k > thr || (k == thr && e < need);
@@ -814,8 +844,8 @@ __device__ __forceinline__ void emit(SelectShared& sh, const Head& a, const uint
         if (s < a.n) {
             if (!keep) a.gaps[s - before] = s;
             else {
-                if (copy) a.mass_out[s] = a.mass[s];
-                if (copy_pos) a.pos_out[s] = a.pos[s];
+                if (copy) a.mass_out[s] = x.mass[i];
+                if (copy_pos) a.pos_out[s] = x.pos[i];
             }
         } else if (keep) a.late[before] = s;         // the move empties it
         else { a.mass_out[s] = 0.f; a.pos_out[s] = -1; }
@@ -837,52 +867,52 @@ __device__ __forceinline__ void keep_all(const Head& a, int64_t from, int64_t to
     }
 }
 
-// A head of one workgroup: a wave holds `per` rows of 64 consecutive slots, their keys in registers.
+// Keys that share the threshold's first digit, from x into list (n of them so far), one wave's after another's.
+template <int R>
+__device__ __forceinline__ void list_keys(const Head& a, const Slots<R>& x, int per, uint32_t digit, uint32_t* list, int* n) {
+    const int lane = threadIdx.x & 63;
+    for_rows<R>(per, [&](auto i) INLINE {
+        const uint32_t k = x.key(a, i, per);
+        const bool in = k != 0u && k >> 21 == digit;
+        const unsigned long long who = __ballot(in);
+        if (who) {
+            int at = 0;
+            if (lane == 0) at = atomicAdd(n, __popcll(who));
+            at = __builtin_amdgcn_readfirstlane(at);
+            if (in) list[at + __popcll(who & ((1ull << lane) - 1))] = k;
+        }
+    });
+}
+
+// A head of one workgroup.
 template <int R>
 __device__ __forceinline__ void select_head(SelectShared& sh, Head& a, int recent) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (a.len + EV_THREADS - 1) / EV_THREADS, s0 = wave * per * 64 + lane;
-    const int stop = min(a.len, (wave + 1) * per * 64);        // slots of this wave
+    const int per = (a.len + EV_THREADS - 1) / EV_THREADS;
+    Slots<R> x;
+    x.load(a, wave * per * 64 + lane, min(a.len, (wave + 1) * per * 64), per);
     if (tid == 0) { sh.newest = -0x7fffffff - 1; sh.listed = 0; }
     clear_hist(sh);
     __syncthreads();
-    if (a.recent) {
-        newest_of(sh, a.pos, s0, stop);
-        a.border = (int64_t)sh.newest - recent;
-    }
-    uint32_t keys[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) keys[i] = 0u;
-    if (wave * per * 64 < a.len) for_rows<R>(per, [&](int i) { keys[i] = i < per ? a.key(s0 + 64 * i, stop) : 0u; });
-    for_rows<R>(per, [&](int i) { count_digit(sh, keys[i] != 0u, keys[i] >> 21); });
+    if (recent > 0) a.protect(block_max(sh, x.newest(per)), recent);
+    for_rows<R>(per, [&](auto i) INLINE { const uint32_t k = x.key(a, i, per); count_digit(sh, k != 0u, k >> 21); });
     __syncthreads();
     pick_digit(sh, a.n);
     uint32_t thr = sh.digit << 21;
     int need = sh.left;
     const bool few = sh.same <= EV_LIST;
     clear_hist(sh);
-    if (few) {
-        // few enough keys share the first digit to look at them alone from here on
-        for_rows<R>(per, [&](int i) {
-            const bool in = keys[i] != 0u && keys[i] >> 21 == thr >> 21;
-            const unsigned long long who = __ballot(in);
-            if (who) {
-                int at = 0;
-                if (lane == 0) at = atomicAdd(&sh.listed, __popcll(who));
-                at = __builtin_amdgcn_readfirstlane(at);
-                if (in) sh.list[at + __popcll(who & ((1ull << lane) - 1))] = keys[i];
-            }
-        });
-    }
+    if (few) list_keys<R>(a, x, per, thr >> 21, sh.list, &sh.listed);      // only these are looked at from here on
     __syncthreads();
     if (few)
-        pick_rest(sh, [&](auto f) { for (int i = tid; i - lane < sh.listed; i += EV_THREADS) f(i < sh.listed ? sh.list[i] : 0u); }, &thr, &need);
-    else pick_rest(sh, [&](auto f) { for_rows<R>(per, [&](int i) { f(keys[i]); }); }, &thr, &need);
-    emit<R>(sh, a, keys, 0, per, stop, thr, need, 0, 0);
+        pick_rest(sh, [&](auto f) INLINE { for (int i = tid; i - lane < sh.listed; i += EV_THREADS) f(i < sh.listed ? sh.list[i] : 0u); }, &thr, &need);
+    else pick_rest(sh, [&](auto f) INLINE { for_rows<R>(per, [&](auto i) INLINE { f(x.key(a, i, per)); }); }, &thr, &need);
+    emit<R>(sh, a, x, per, thr, need, 0, 0);
 }
 
 // One workgroup per (sequence, kv head). The n-th greatest key by a radix select of 11 + 11 + 10 bits, then one pass in
-// slot order. The keys stay in registers, so masses are read once and positions twice; what is left are LDS counters.
+// slot order. Masses and positions stay in registers, so they are read once, together; what is left are LDS counters and a
+// dozen barriers.
 __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, const KvTable tb, const KvEvict a) {
     __shared__ SelectShared sh;
     Head head(p, tb, a, blockIdx.x, blockIdx.y, blockIdx.x == 0 && threadIdx.x == 0);
@@ -901,7 +931,7 @@ struct ChunkWork {
     int32_t* newest;                     // [chunks]
     uint32_t* hist;                      // [chunks][2048]
     uint32_t* list;                      // [chunks][EV_CHUNK]
-    __device__ ChunkWork(const KvEvict& a, int64_t row, int chunks) {
+    __device__ __forceinline__ ChunkWork(const KvEvict& a, int64_t row, int chunks) {
         newest = a.chunk_newest + row * chunks;
         hist = a.chunk_hist + row * chunks * 2048;
         list = a.chunk_list + row * chunks * EV_CHUNK;
@@ -916,28 +946,28 @@ __global__ __launch_bounds__(EV_THREADS) void kv_select_chunk_kernel(const KvPoo
     const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     Head head(p, tb, a, h, b, STAGE == 3 && c == 0 && h == 0 && tid == 0);
     const ChunkWork ws(a, (int64_t)b * p.heads + h, gridDim.x);
-    const int slot0 = c * EV_CHUNK, s0 = slot0 + wave * (EV_CHUNK / EV_WAVES) + lane;
-    const int stop = min(head.len, slot0 + (wave + 1) * (EV_CHUNK / EV_WAVES));
-    const int chunks = (head.len + EV_CHUNK - 1) / EV_CHUNK;
+    const int slot0 = c * EV_CHUNK, chunks = (head.len + EV_CHUNK - 1) / EV_CHUNK;
     if (STAGE == 3) keep_all(head, slot0, c + 1 == (int)gridDim.x ? a.side_ld : min<int64_t>(a.side_ld, slot0 + EV_CHUNK));
     if (head.len <= head.n || c >= chunks) return;
     if (tid == 0) { sh.newest = -0x7fffffff - 1; sh.listed = 0; }
     clear_hist(sh);
+    Slots<R> x;
+    const int s0 = slot0 + wave * R * 64;
+    x.load(head, s0 + lane, min(head.len, s0 + R * 64), R);
     __syncthreads();
     if (STAGE == 0) {
-        newest_of(sh, head.pos, s0, stop);
-        if (tid == 0) ws.newest[c] = sh.newest;
+        const int newest = block_max(sh, x.newest(R));
+        if (tid == 0) ws.newest[c] = newest;
         return;
     }
-    if (head.recent) {
-        newest_of(sh, ws.newest, tid, wave == 0 ? chunks : 0);
-        head.border = (int64_t)sh.newest - a.recent;
+    if (a.recent > 0) {
+        int newest = -0x7fffffff - 1;
+        if (wave == 0)
+            for (int i = lane; i < chunks; i += 64) newest = max(newest, ws.newest[i]);
+        head.protect(block_max(sh, newest), a.recent);
     }
-    uint32_t keys[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) keys[i] = s0 - lane < stop ? head.key(s0 + 64 * i, stop) : 0u;
     if (STAGE == 1) {
-        for_rows<R>(R, [&](int i) { count_digit(sh, keys[i] != 0u, keys[i] >> 21); });
+        for_rows<R>(R, [&](auto i) INLINE { const uint32_t k = x.key(head, i, R); count_digit(sh, k != 0u, k >> 21); });
         __syncthreads();
         for (int i = tid; i < 2048; i += EV_THREADS) ws.hist[(int64_t)c * 2048 + i] = sh.hist[i];
         return;
@@ -956,34 +986,45 @@ __global__ __launch_bounds__(EV_THREADS) void kv_select_chunk_kernel(const KvPoo
     pick_digit(sh, head.n, c0, c1);
     const uint32_t digit = sh.digit;
     if (STAGE == 2) {
-        for_rows<R>(R, [&](int i) {
-            const bool in = keys[i] != 0u && keys[i] >> 21 == digit;
-            const unsigned long long who = __ballot(in);
-            if (who) {
-                int at = 0;
-                if (lane == 0) at = atomicAdd(&sh.listed, __popcll(who));
-                at = __builtin_amdgcn_readfirstlane(at);
-                if (in) ws.list[(int64_t)c * EV_CHUNK + at + __popcll(who & ((1ull << lane) - 1))] = keys[i];
-            }
-        });
+        list_keys<R>(head, x, R, digit, ws.list + (int64_t)c * EV_CHUNK, &sh.listed);
         return;
     }
     uint32_t thr = digit << 21;
     int need = sh.left;
+    const int same = sh.same;
     int gt = block_sum(sh, (top > (int)digit ? l0 : 0) + (top - 1 > (int)digit ? l1 : 0));
-    // the keys that share it, chunk by chunk
-    auto each = [&](int upto, auto f) {
-        for (int i = 0; i < upto; ++i) {
-            const int n = (int)ws.hist[(int64_t)i * 2048 + digit];
-            for (int j = tid; j - lane < n; j += EV_THREADS) f(j < n ? ws.list[(int64_t)i * EV_CHUNK + j] : 0u);
+    // The keys that share the digit, chunk by chunk: out of LDS where they fit (chunk i's are list[i's predecessors' ..], a
+    // chunk per wave at a time), else again and again out of the workspace.
+    int before = 0;                                  // of them, those of chunks before this one
+    if (same <= EV_LIST) {
+        int sum = 0;
+        for (int i0 = 0; i0 < chunks; i0 += 64) {
+            const int n = i0 + lane < chunks ? (int)ws.hist[(int64_t)(i0 + lane) * 2048 + digit] : 0, inc = wave_scan(n);
+            for (int i = wave; i < 64; i += EV_WAVES) {
+                const int m = __builtin_amdgcn_readlane(n, i), to = sum + __builtin_amdgcn_readlane(inc - n, i);
+                for (int j = lane; j < m; j += 64) sh.list[to + j] = ws.list[(int64_t)(i0 + i) * EV_CHUNK + j];
+            }
+            if (i0 <= c && c < i0 + 64) before = sum + __builtin_amdgcn_readlane(inc - n, c - i0);
+            sum += __builtin_amdgcn_readlane(inc, 63);
+        }
+        __syncthreads();
+    }
+    auto each = [&](int upto, int upto_keys, auto f) INLINE {
+        if (same <= EV_LIST) {
+            for (int j = tid; j - lane < upto_keys; j += EV_THREADS) f(j < upto_keys ? sh.list[j] : 0u);
+        } else {
+            for (int i = 0; i < upto; ++i) {
+                const int n = (int)ws.hist[(int64_t)i * 2048 + digit];
+                for (int j = tid; j - lane < n; j += EV_THREADS) f(j < n ? ws.list[(int64_t)i * EV_CHUNK + j] : 0u);
+            }
         }
     };
-    pick_rest(sh, [&](auto f) { each(chunks, f); }, &thr, &need);
+    pick_rest(sh, [&](auto f) INLINE { each(chunks, same, f); }, &thr, &need);
     int g = 0, e = 0;
-    each(c, [&](uint32_t k) { g += k > thr; e += k == thr; });
+    each(c, before, [&](uint32_t k) INLINE { g += k > thr; e += k == thr; });
     gt += block_sum(sh, g);
     const int eq = block_sum(sh, e);
-    emit<R>(sh, head, keys, slot0, EV_CHUNK / EV_THREADS, stop, thr, need, gt, eq);
+    emit<R>(sh, head, x, R, thr, need, gt, eq);
 }
 
 // Row late[kept_low + i] -> row gaps[i], K and V and the side tables. Sources lie at n and beyond, targets below it.
