@@ -143,6 +143,14 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_max(int x) { return max(x, __builtin_amdgcn_update_dpp(-0x7fffffff - 1, x, CTRL, ROWS, 0xf, false)); }
+
+__device__ __forceinline__ int wave_max(int x) {
+    x = dpp_max<0x118, 0xf>(dpp_max<0x114, 0xf>(dpp_max<0x112, 0xf>(dpp_max<0x111, 0xf>(x))));
+    return __builtin_amdgcn_readlane(dpp_max<0x143, 0xc>(dpp_max<0x142, 0xa>(x)), 63);
+}
+
 // f over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48), for each of them.
 template <class F>
 __device__ __forceinline__ float column_all(float x, F f) {
@@ -761,11 +769,7 @@ __device__ __forceinline__ int block_sum(SelectShared& sh, int x) {
 // 2047 - 2 tid and 2046 - 2 tid. Ends with a barrier.
 __device__ __forceinline__ void pick_digit(SelectShared& sh, int want, int c0, int c1) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, top = 2047 - 2 * tid;
-    int inc = c0 + c1;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(inc, o);
-        if (lane >= o) inc += x;
-    }
+    int inc = wave_scan(c0 + c1);
     if (lane == 63) sh.wave_a[wave] = inc;
     __syncthreads();
     for (int w = 0; w < EV_WAVES; ++w) inc += w < wave ? sh.wave_a[w] : 0;
@@ -804,7 +808,7 @@ __device__ __forceinline__ void pick_rest(SelectShared& sh, E each, uint32_t* th
 
 // Greatest of x over the workgroup, in sh.newest (set to the least before). Ends with a barrier.
 __device__ __forceinline__ int block_max(SelectShared& sh, int x) {
-    for (int o = 32; o; o >>= 1) x = max(x, __shfl_xor(x, o));
+    x = wave_max(x);
     if ((threadIdx.x & 63) == 0) atomicMax(&sh.newest, x);
     __syncthreads();
     return sh.newest;
@@ -1150,8 +1154,8 @@ static size_t kv_evict_list(const KvPool& p, int max_pages, int budget) {
     return (size_t)std::min<int64_t>(budget, (int64_t)max_pages << p.page_shift);
 }
 
-// Chunks of the long select, 0 where a workgroup holds a head. (One launch against four: an eviction of 32 heads takes 30
-// us and 45 at 8192 slots, 39 and 45 at 16384; at 65536 a workgroup a head took 168, the chunks 79.)
+// Chunks of the long select, 0 where a workgroup holds a head. (One launch against four: an eviction of 32 heads takes 25
+// us and 37 at 8192 slots, 32 and 37 at 16384; at 65536 a workgroup a head took 168, the chunks take 65.)
 static int64_t kv_evict_chunks(const KvPool& p, int max_pages) {
     const int64_t cap = (int64_t)max_pages << p.page_shift;
     return cap <= EV_ROWS * EV_THREADS ? 0 : (cap + EV_CHUNK - 1) / EV_CHUNK;
