@@ -10,7 +10,7 @@ base=${src%.hip}
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function "$@" \
     -c tacotron_amd/csrc/${VSRC:-$src} -o $o/${base}_$name.o
 objs=""
-for f in api gemm rnn decoder dec_persistent dec_tile griffinlim; do
+for f in api gemm rnn decoder dec_persistent dec_tile griffinlim kv_cache; do
   if [ "$f" = "$base" ]; then objs="$objs $o/${base}_$name.o"; else objs="$objs $o/$f.o"; fi
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o tacotron_amd/libtaco_v_$name.so $objs
