@@ -1735,7 +1735,7 @@ extern "C" int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int6
                T, starts, counts, first, mass, positions, side_ld, lengths_out};
     if (int rc = kv_rows(what, p, k, a.k_st, 3)) return rc;
     if (int rc = kv_rows(what, p, v, a.v_st, 3)) return rc;
-    if (T < 1 || (int64_t)T * p.heads > (1 << 26)) return fail("%s: T must be at least 1 and T * kv_heads at most 2^26 (got T %d)", what, T);
+    if (T < 1 || (int64_t)T * p.heads > (1 << 25)) return fail("%s: T must be at least 1 and T * kv_heads at most 2^25 (got T %d)", what, T);
     if (!starts || !lengths_out) return fail("%s: null argument", what);
     if (mass || positions)
         if (int rc = kv_side(what, p, t, side_ld)) return rc;

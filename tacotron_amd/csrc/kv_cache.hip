@@ -16,6 +16,7 @@ namespace {
 
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // a lambda that is not inlined would keep the registers it refers to in memory
 #define INLINE __attribute__((always_inline))
@@ -38,8 +39,13 @@ __device__ __forceinline__ int64_t slot_off(const int64_t* st, int page, int h, 
 // ---------------------------------------------------------------------------------------
 // append
 
-// Copies 16 bytes per lane: planes 0 / 1 of the grid are K / V, (t, h, 16-byte column) with the column fastest; plane 2
-// the side tables, (h, t) with t fastest. Nothing but the copy bounds it: the rows come in once and go out once.
+// 16-byte pieces per lane. (8 x 4097 tokens of 8 heads, bf16, take 50 us with 2, 49 with 4, 62 with 1 and through the caches;
+// 32 x 150 of one head, fp32, 6.6, 8.0 and 7.1.)
+constexpr int AP_ITEMS = 2;
+
+// Planes 0 / 1 of the grid copy K / V, 16-byte pieces (t, h, column) with the column fastest, AP_ITEMS per lane, all read
+// before the first is written; plane 2 writes the side tables, (h, t) with t fastest. Nothing but the copy bounds it: rows
+// come in once and go out once, past the caches.
 __global__ __launch_bounds__(256) void kv_append_kernel(const KvPool p, const KvTable tb, const KvAppend a) {
     const int b = blockIdx.y, plane = blockIdx.z;
     const int cap = tb.max_pages << p.page_shift;
@@ -51,32 +57,41 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvPool p, const Kv
         if (first_thread) atomicOr(p.status, KV_BAD_LENGTH);
     }
     if (first_thread) a.lengths_out[b] = start + count;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (plane == 2) {
-        if (i >= (int64_t)p.heads * a.T) return;
-        const int t = (int)(i % a.T), h = (int)(i / a.T);
-        if (t >= count) return;
-        const int64_t o = ((int64_t)b * p.heads + h) * a.side_ld + start + t;
-        if (a.mass) a.mass[o] = 0.f;
-        if (a.positions) a.positions[o] = (a.first ? a.first[b] : start) + t;
+        const uint32_t n = (uint32_t)p.heads * (uint32_t)a.T;
+        for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
+            const int t = (int)(i % a.T), h = (int)(i / a.T);
+            if (t >= count) continue;
+            const int64_t o = ((int64_t)b * p.heads + h) * a.side_ld + start + t;
+            if (a.mass) a.mass[o] = 0.f;
+            if (a.positions) a.positions[o] = (a.first ? a.first[b] : start) + t;
+        }
         return;
     }
-    const int vecs = (p.dim * p.esize) >> 4;
-    if (i >= (int64_t)a.T * p.heads * vecs) return;
-    const int c = (int)(i % vecs);
-    const int64_t th = i / vecs;
-    const int h = (int)(th % p.heads), t = (int)(th / p.heads);
-    if (t >= count) return;
-    const int s = start + t;
-    const int page = tb.table[(int64_t)b * tb.ld + (s >> p.page_shift)];
-    if ((unsigned)page >= (unsigned)p.num_pages) {
-        if (c == 0) atomicOr(p.status, KV_BAD_PAGE);
-        return;
-    }
+    const int vec_shift = 31 - __builtin_clz((p.dim * p.esize) >> 4);      // pieces per row: a power of two
+    const uint32_t n = ((uint32_t)count * (uint32_t)p.heads) << vec_shift;
+    const uint32_t i0 = blockIdx.x * (256 * AP_ITEMS) + threadIdx.x;
+    if (i0 >= n) return;
     const int64_t* xs = plane ? a.v_st : a.k_st;
-    const char* src = (const char*)(plane ? a.v : a.k) + ((int64_t)b * xs[0] + (int64_t)t * xs[1] + (int64_t)h * xs[2]) * p.esize;
-    char* dst = (char*)(plane ? p.v : p.k) + slot_off(plane ? p.v_st : p.k_st, page, h, s & (p.page_size - 1)) * p.esize;
-    reinterpret_cast<uint4*>(dst)[c] = reinterpret_cast<const uint4*>(src)[c];
+    const int64_t* ps = plane ? p.v_st : p.k_st;
+    const char* src = (const char*)(plane ? a.v : a.k) + (int64_t)b * xs[0] * p.esize;
+    char* dst = (char*)(plane ? p.v : p.k);
+    const int32_t* row = tb.table + (int64_t)b * tb.ld;
+    u32x4 x[AP_ITEMS];
+    int64_t to[AP_ITEMS];
+#pragma unroll
+    for (int j = 0; j < AP_ITEMS; ++j) {
+        const uint32_t i = min(i0 + 256 * j, n - 1), th = i >> vec_shift;      // (behind the end: the last piece, not written)
+        const int c = (int)(i & ((1u << vec_shift) - 1)), t = (int)(th / (uint32_t)p.heads), h = (int)(th - (uint32_t)t * p.heads), s = start + t;
+        const int page = row[s >> p.page_shift];
+        to[j] = -1;
+        if ((unsigned)page >= (unsigned)p.num_pages) atomicOr(p.status, KV_BAD_PAGE);
+        else if (i0 + 256 * j < n) to[j] = slot_off(ps, page, h, s & (p.page_size - 1)) * p.esize + 16 * c;
+        x[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + ((int64_t)t * xs[1] + (int64_t)h * xs[2]) * p.esize + 16 * c));
+    }
+#pragma unroll
+    for (int j = 0; j < AP_ITEMS; ++j)
+        if (to[j] >= 0) __builtin_nontemporal_store(x[j], reinterpret_cast<u32x4*>(dst + to[j]));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -108,7 +123,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvPool p, const Kv
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int AT_WAVES = 4;
@@ -1082,9 +1096,9 @@ static int kv_cus(int device) {
 }
 
 void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hipStream_t s) {
-    const int64_t copies = (int64_t)a.T * p.heads * ((p.dim * p.esize) >> 4);
+    const int64_t pieces = (int64_t)a.T * p.heads * ((p.dim * p.esize) >> 4);
     const bool side = a.mass || a.positions;
-    kv_append_kernel<<<dim3((unsigned)((copies + 255) / 256), tb.B, side ? 3 : 2), 256, 0, s>>>(p, tb, a);
+    kv_append_kernel<<<dim3((unsigned)((pieces + 256 * AP_ITEMS - 1) / (256 * AP_ITEMS)), tb.B, side ? 3 : 2), 256, 0, s>>>(p, tb, a);
 }
 
 // Tiles of the line if every sequence filled its table.
