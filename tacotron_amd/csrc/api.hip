@@ -1768,7 +1768,7 @@ extern "C" int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int6
                nullptr, nullptr, nullptr, 0};
     if (int rc = kv_rows(what, p, q, a.q_st, 2)) return rc;
     if (!lengths || !out || !lse || !aligned16(out)) return fail("%s: null argument, or out not on a 16-byte boundary", what);
-    if (!std::isfinite(scale)) return fail("%s: scale must be finite", what);
+    if (!std::isfinite(a.scale2)) return fail("%s: scale (and scale * log2(e)) must be finite", what);
     if (mass)
         if (int rc = kv_side(what, p, t, side_ld)) return rc;
     if (!ws || !aligned16(ws) || ws_bytes < kv_attend_ws_bytes(p, B, a.group, max_pages, mass != nullptr))

@@ -87,7 +87,8 @@ def test_pools_that_are_refused(bad, text):
     (_append, dict(mass=16, side_ld=63), 'side'), (_append, dict(positions=16, side_ld=63), 'side'),
     (_attend, dict(q_heads=3), 'q_heads'), (_attend, dict(q_heads=0), 'q_heads'), (_attend, dict(q=None), 'null'), (_attend, dict(q=24), 'boundary'),
     (_attend, dict(out=None), 'null'), (_attend, dict(out=20), 'boundary'), (_attend, dict(lse=None), 'null'),
-    (_attend, dict(lengths=None), 'null'), (_attend, dict(scale=float('nan')), 'scale'), (_attend, dict(scale=float('inf')), 'scale'),
+    (_attend, dict(lengths=None), 'null'), (_attend, dict(scale=float('nan')), 'scale'), (_attend, dict(scale=float('inf')), 'scale'), (_attend, dict(scale=3e38), 'scale'), (_attend, dict(B=65535, q_heads=65534), 'too many'),
+    (_attend, dict(B=65535, max_pages=1 << 20, table_ld=1 << 20), 'too many'),
     (_attend, dict(mass=16, side_ld=32), 'side'), (_attend, dict(ws=None), 'workspace'),
     (_evict, dict(budget=0), 'budget'), (_evict, dict(recent=-1), 'recent'), (_evict, dict(recent=9), 'recent'),
     (_evict, dict(side_ld=10), 'side'), (_evict, dict(mass=None), 'null'), (_evict, dict(po=None), 'null'),

@@ -450,6 +450,39 @@ def test_evict_long(inplace):
     _check_evict(cache, table, lengths, mass, pos, 8192, 100, inplace)
 
 
+@pytest.mark.parametrize('inplace', [False, True])
+def test_evict_shared_by_workgroups(inplace):
+    """Tables past what one workgroup holds: rows under the budget and empty ones among long ones, every kind of mass, a
+    budget in the middle of a stretch, more stretches than a wave has lanes."""
+    import torch
+    lens = [70003, 100, 0, 40000, 39999, 8192, 16385]
+    cache, table, lengths = _make(47, lens, 2, 64, 128, 'float16')
+    slots = table.shape[1] * 128 + 3
+    g = torch.Generator().manual_seed(2)
+    mass = torch.rand(len(lens), 2, slots, generator=g) ** 3
+    pick = torch.rand(mass.shape, generator=g)
+    mass[pick < 0.05] = 0.0
+    mass[(pick > 0.1) & (pick < 0.15)] = float('nan')
+    mass[(pick > 0.2) & (pick < 0.25)] = float('inf')
+    mass[(pick > 0.3) & (pick < 0.5)] = 0.125
+    mass[(pick > 0.6) & (pick < 0.7)] *= -1
+    pos = torch.stack([torch.stack([torch.randperm(slots, generator=g) for _ in range(2)]) for _ in lens]).to(torch.int32)
+    _check_evict(cache, table, lengths, mass.cuda(), pos.cuda(), 39999, 5000, inplace)
+
+
+def test_evict_more_stretches_than_lanes():
+    import torch
+    lens = [600001]
+    cache, table, lengths = _make(49, lens, 1, 64, 256, 'bfloat16')
+    slots = table.shape[1] * 256
+    g = torch.Generator().manual_seed(3)
+    pos = torch.arange(slots, dtype=torch.int32).view(1, 1, slots).cuda()
+    _check_evict(cache, table, lengths, torch.rand(1, 1, slots, generator=g).cuda(), pos, 100000, 64, False)
+    cache, table, lengths = _make(49, lens, 1, 64, 256, 'bfloat16')
+    mass = torch.floor(torch.rand(1, 1, slots, generator=g) * 3).cuda()
+    _check_evict(cache, table, lengths, mass, pos, 300000, 0, False)
+
+
 def test_evict_bad_pages_move_nothing_there():
     import torch
     from tacotron_amd.engine import TacoError
@@ -630,6 +663,37 @@ def test_calls_on_several_streams():
         for r in got[i]:
             for a, b in zip(r, want[i]):
                 assert torch.equal(a, b)
+
+
+def test_other_streams_and_captured_graphs_share_nothing():
+    """Two captured attends of different sizes, replayed in turn and beside an eager one on another stream."""
+    import torch
+    cases = []
+    for i, lens in enumerate(([700, 31, 2500], [64, 9000])):
+        cache, table, lengths = _make(73 + i, lens, 2, 64, 16, 'bfloat16')
+        q = _q(75 + i, len(lens), 6, 64, 'bfloat16')
+        mass = torch.zeros(len(lens), 2, table.shape[1] * 16, device='cuda')
+        want = (*cache.attend(q, table, lengths, mass=mass), mass)
+        graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(mass)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            out.zero_()
+            got = (*cache.attend(q, table, lengths, mass=out), out)
+        cases.append((cache, table, lengths, q, want, graph, got))
+    side = torch.cuda.Stream()
+    for turn in range(6):
+        order = cases if turn % 2 else cases[::-1]
+        for c in order:
+            c[5].replay()
+        with torch.cuda.stream(side):
+            eager = cases[turn % 2]
+            out, lse = eager[0].attend(eager[3], eager[1], eager[2])
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[4][0]) and torch.equal(lse, eager[4][1])
+        for c in cases:
+            for a, b in zip(c[6], c[4]):
+                assert torch.equal(a, b), turn
+        torch.zeros(1 << 20, device='cuda').add_(1)
 
 
 def test_encoder_memory(engine, hp):
