@@ -104,9 +104,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvPool p, const Kv
 // are one line, and wave w of W takes the w-th W-th of it. The line is laid out on the device from the lengths, so the
 // split follows the lengths that are there when the kernel (or a captured graph) runs, a ragged batch is as balanced as
 // an even one, and one long sequence fills the chip. A wave walks its share tile by tile, from one head into the next, with
-// the next tile's K always in flight, and meets no barrier; four waves to a CU keep enough loads in flight (64 KB), and more
-// of them only spread the reads over more pages at a time. Heads that end up in several waves leave {maximum, sum,
-// unnormalised output} of each in the workspace and kv_join_kernel joins them.
+// the next tile's K always in flight, and meets no barrier; four waves to a CU keep enough loads in flight (64 KB; eight at
+// D = 64). Heads that end up in several waves leave {maximum, sum, unnormalised output} of each in the workspace and
+// kv_join_kernel joins them.
 //
 // Products. Query heads of one kv head are the columns of 16-wide tiles (a group over 16 takes several passes, one under
 // 16 leaves columns idle: the matrix cores have the room, the reads of K and V are what counts).
@@ -127,6 +127,11 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int AT_WAVES = 4;
 
+// Workgroups to a CU, which share its 160 KB of LDS. A tile of D = 64 is half as much to have in flight: two (32 x 16384
+// tokens of 8 heads: 188 us with one, 169 with two, 174 with three). Above, a second one costs more in parts to join than it
+// brings (64 heads over 4 of 128, 64 x 4096: 65 us with one, 73 with two).
+constexpr int attend_per_cu(int dim) { return dim == 64 ? 2 : 1; }
+
 template <int DT, int D>
 struct AttendShape {
     static constexpr int ES = DT == KV_F32 ? 4 : 2;
@@ -135,10 +140,8 @@ struct AttendShape {
     static constexpr int NX = D / (16 * VEC);
     static constexpr int NACC = D / 16;
     static constexpr int KL = D * ES / 64;                     // 16-byte loads per lane and K row
+    static constexpr int GATHER = 39 * 1024 / attend_per_cu(D);        // bytes of scores a wave gathers in LDS
 };
-
-// Bytes of scores a wave gathers in LDS: the workgroup's four share the CU's 160 KB.
-constexpr int AT_GATHER = 39 * 1024;
 
 int attend_tile(int dtype) { return dtype == KV_F32 ? AttendShape<KV_F32, 64>::TW : AttendShape<KV_BF16, 64>::TW; }
 
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
     // many small weights beside a large one are not lost
     constexpr float OFF = DT == KV_F16 ? 14.f : 0.f;
     typedef typename std::conditional<VEC * ES == 16, u32x4, u32x2>::type vload_t;
-    __shared__ f32x4 gathered[MASS ? AT_WAVES : 1][MASS ? AT_GATHER / 16 : 1];
+    __shared__ f32x4 gathered[MASS ? AT_WAVES : 1][MASS ? S::GATHER / 16 : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
@@ -340,7 +343,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
     // Scores for the weights of `mass`: [tile][score_rows][TW]. A wave gathers those of tiles gather0, gather0 + 1, ... and
     // writes them out when there is room for no more, and at the end: a trickle of writes among the reads costs far more of
     // the memory's time than their bytes.
-    const int tile_vecs = a.score_rows * TW / 4, room = AT_GATHER / 16 / tile_vecs;
+    const int tile_vecs = a.score_rows * TW / 4, room = S::GATHER / 16 / tile_vecs;
     int gather0 = u0;
     auto flush = [&](int upto) {
         f32x4* to = (f32x4*)a.scores + (int64_t)gather0 * tile_vecs;
@@ -1114,9 +1117,10 @@ bool kv_attend_fits(const KvPool& p, int B, int group, int max_pages) {
            (int64_t)B * p.heads * (group + (cap + 1023) / 1024) < (1ll << 24);
 }
 
-// Workgroups of the attention: one to a CU, or a tile for every wave where there are fewer.
+// Workgroups of the attention: as many as the CUs hold, or a tile for every wave where there are fewer.
 static int attend_groups(const KvPool& p, int B, int group, int max_pages) {
-    return (int)std::min<int64_t>((attend_tiles(p, B, group, max_pages) + AT_WAVES - 1) / AT_WAVES, kv_cus(p.device));
+    return (int)std::min<int64_t>((attend_tiles(p, B, group, max_pages) + AT_WAVES - 1) / AT_WAVES,
+                                  attend_per_cu(p.dim) * kv_cus(p.device));
 }
 
 // {maximum, sum} and output of two parts per wave (the one it begins with, the one it ends with), and the scores
