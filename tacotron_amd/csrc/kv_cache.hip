@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
             f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
             for (int c = 0; c < nh; ++c) {           // (tiles are multiples of 4 tokens: four scores lie together)
-                const f32x4 x = *reinterpret_cast<const f32x4*>(s + c * tw);
+                const f32x4 x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(s + c * tw));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] += ex2(x[e] - lse2[c]);
             }
