@@ -628,6 +628,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         return;
     }
     float* mass = a.mass + ((int64_t)b * p.heads + kvh) * a.side_ld;
+    const bool whole4 = ((uintptr_t)mass & 15) == 0;
     for (int g = 0; g < ngrp; ++g) {
         const Parts q = parts_of(g);
         const int nh = min(16, a.group - 16 * g);
@@ -651,9 +652,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] += ex2(x[e] - lse2[c]);
             }
+            if (whole4 && t + 4 <= len) *reinterpret_cast<f32x4*>(mass + t) += sum;
+            else
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (t + e < len) mass[t + e] += sum[e];
+                for (int e = 0; e < 4; ++e)
+                    if (t + e < len) mass[t + e] += sum[e];
         }
         __syncthreads();
     }
