@@ -273,7 +273,7 @@ struct KvAttend {
     float scale2;                         // scale * log2(e): scores are kept in units of ln 2
     void* out; float* lse;                // contiguous
     float* mass; int64_t side_ld;
-    // workspace: parts of heads that several waves share, [2 * waves][16] {maximum, sum} and
+    // workspace: parts of heads that several waves share, [2 * waves][16 or 32 heads] {maximum, sum} and
     // [2 * waves][score_rows][dim]; with mass, the scores, [tiles][score_rows][a tile's tokens]
     float2* part_ml; float* part_out; float* scores; int score_rows;
 };

@@ -108,8 +108,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvPool p, const Kv
 // D = 64). Heads that end up in several waves leave {maximum, sum, unnormalised output} of each in the workspace and
 // kv_join_kernel joins them.
 //
-// Products. Query heads of one kv head are the columns of 16-wide tiles (a group over 16 takes several passes, one under
-// 16 leaves columns idle: the matrix cores have the room, the reads of K and V are what counts).
+// Products. Query heads of one kv head are the columns of a 16-wide tile, or of two where a group has more than 16 (one over
+// 32 takes several passes over K and V). A group under 16 leaves columns idle: the matrix cores have the room, the reads
+// of K and V are what counts.
 //   S^T = K Q^T: a lane of the A operand is a token (lane & 15) with 16 bytes of its row at 16 (lane >> 4) + 64 j; the
 //     order of the summed dimension is free as long as Q has the same, so both are plain 16-byte loads.
 //   O^T += V^T P^T: the C layout of S^T leaves lane (g = lane >> 4, head = lane & 15) with rows 4 g + i of every 16, which
@@ -131,6 +132,13 @@ constexpr int AT_WAVES = 4;
 // tokens of 8 heads: 188 us with one, 169 with two, 174 with three). Above, a second one costs more in parts to join than it
 // brings (64 heads over 4 of 128, 64 x 4096: 65 us with one, 73 with two).
 constexpr int attend_per_cu(int dim) { return dim == 64 ? 2 : 1; }
+
+// Query heads of a group that one pass over K and V serves: 32 where there are more than 16 (32 heads over one of 128, 32 x
+// 8192 tokens, bf16: 32 us in one pass, 39 in two), but at fp32 and D = 256, where two tiles' sums do not fit the registers
+// (124 us against 119).
+__host__ __device__ constexpr int attend_columns(int dtype, int dim, int group) { return group > 16 && !(dtype == KV_F32 && dim == 256) ? 32 : 16; }
+static int attend_columns(const KvPool& p, int group) { return attend_columns(p.dtype, p.dim, group); }
+static int attend_passes(const KvPool& p, int group) { return (group + attend_columns(p, group) - 1) / attend_columns(p, group); }
 
 template <int DT, int D>
 struct AttendShape {
@@ -237,11 +245,12 @@ struct Cursor {
     int nb, len;                         // tiles and tokens of the sequence
 };
 
-template <int DT, int D, bool MASS>
+template <int DT, int D, bool MASS, int NG>
 __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
     using S = AttendShape<DT, D>;
     constexpr int TW = S::TW, VEC = S::VEC, NX = S::NX, NACC = S::NACC, KL = S::KL, ES = S::ES;
     constexpr int NS = TW / 16, NV = TW / 4;         // 16-token blocks; tokens a lane holds, NV (lane >> 4) and on
+    constexpr int COLS = 16 * NG;                    // a lane has heads col + 16 g of the group's stretch, g < NG
     // fp16 weights are kept 2^14 too large (the sums with them): at most 16384, and 2^-28 is still a normal number, so that
     // many small weights beside a large one are not lost
     constexpr float OFF = DT == KV_F16 ? 14.f : 0.f;
@@ -252,7 +261,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
     const int col = lane & 15, grp = lane >> 4;
     const int ktok = NS == 2 ? 8 * (col >> 2) + (col & 3) : col;     // token of this lane's K row, block 0
     const int cap = tb.max_pages << p.page_shift, w = blockIdx.x * AT_WAVES + wave;
-    const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
+    const int ngrp = (a.group + COLS - 1) / COLS, H = p.heads * ngrp, hq = p.heads * a.group;
 
     // the line, from the tiles of the first 64 sequences (a lane each; their lengths stay at hand) and, 64 by 64, the rest
     auto tiles = [](int len) { return (len + TW - 1) / TW; };
@@ -321,7 +330,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
     auto page_of = [&](const Cursor& c, int t) { return tb.table[(int64_t)c.b * tb.ld + (min(c.tile * TW + t, c.len - 1) >> p.page_shift)]; };
     auto bad_id = [&](int page) { return (unsigned)page >= (unsigned)p.num_pages; };
     const int mask = p.page_size - 1;
-    u32x4 kf[NS][KL], qf[KL];
+    u32x4 kf[NS][KL], qf[NG][KL];
     auto load_k = [&](const Cursor& c, int page) {
         const int kvh = c.hg / ngrp;
         const char* r = (const char*)p.k + ((int64_t)kvh * p.k_st[1] + (int64_t)(bad_id(page) ? 0 : page) * p.k_st[0] +
@@ -332,12 +341,16 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
             for (int j = 0; j < KL; ++j)
                 kf[s][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(r + 4 * s * p.k_st[2] * ES + j * 64));
     };
-    auto head0_of = [&](const Cursor& c) { return c.hg / ngrp * a.group + c.hg % ngrp * 16; };
-    auto heads_of = [&](const Cursor& c) { return min(16, a.group - c.hg % ngrp * 16); };
+    auto head0_of = [&](const Cursor& c) { return c.hg / ngrp * a.group + c.hg % ngrp * COLS; };
+    auto heads_of = [&](const Cursor& c) { return min(COLS, a.group - c.hg % ngrp * COLS); };
     auto load_q = [&](const Cursor& c) {
-        const char* q = (const char*)a.q + ((int64_t)c.b * a.q_st[0] + (int64_t)(head0_of(c) + min(col, heads_of(c) - 1)) * a.q_st[1]) * ES + grp * 16;
 #pragma unroll
-        for (int j = 0; j < KL; ++j) qf[j] = *reinterpret_cast<const u32x4*>(q + j * 64);      // (idle columns: the last head again)
+        for (int g = 0; g < NG; ++g) {
+            const int head = head0_of(c) + min(col + 16 * g, heads_of(c) - 1);      // (idle columns: the last head again)
+            const char* q = (const char*)a.q + ((int64_t)c.b * a.q_st[0] + (int64_t)head * a.q_st[1]) * ES + grp * 16;
+#pragma unroll
+            for (int j = 0; j < KL; ++j) qf[g][j] = *reinterpret_cast<const u32x4*>(q + j * 64);
+        }
     };
 
     // Scores for the weights of `mass`: [tile][score_rows][TW]. A wave gathers those of tiles gather0, gather0 + 1, ... and
@@ -353,10 +366,18 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
         gather0 = upto;
     };
 
-    float m = -INFINITY, l = 0.f;
-    f32x4 acc[NACC];
+    float m[NG], l[NG];
+    f32x4 acc[NG][NACC];
+    auto reset = [&]() INLINE {
 #pragma unroll
-    for (int n = 0; n < NACC; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int g = 0; g < NG; ++g) {
+            m[g] = -INFINITY;
+            l[g] = 0.f;
+#pragma unroll
+            for (int n = 0; n < NACC; ++n) acc[g][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    };
+    reset();
     int vpage = page_of(cur, NV * grp);
     load_q(cur);
     load_k(cur, page_of(cur, ktok));
@@ -379,15 +400,17 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
 #pragma unroll
             for (int x = 0; x < NX; ++x)
                 vf[i][x] = __builtin_nontemporal_load(reinterpret_cast<const vload_t*>(r + i * p.v_st[2] * ES + x * 16 * VEC * ES));
-        float sc[NV];
+        float sc[NG][NV];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            f32x4 c = {0.f, 0.f, 0.f, 0.f};
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int j = 0; j < KL; ++j) c = Mma<DT>::run(kf[s][j], qf[j], c);
+            for (int s = 0; s < NS; ++s) {
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[4 * s + i] = c[i] * a.scale2;
-        }
+                for (int j = 0; j < KL; ++j) c = Mma<DT>::run(kf[s][j], qf[g][j], c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[g][4 * s + i] = c[i] * a.scale2;
+            }
         const bool end = last || next.tile == 0;     // of the head, as far as it is this wave's
         const int nh = heads_of(cur);
         if (!last) {
@@ -400,35 +423,42 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (bad || tok + i >= cur.len) {
-                    sc[i] = -INFINITY;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) sc[g][i] = -INFINITY;
 #pragma unroll
                     for (int x = 0; x < NX; ++x) vf[i][x] = vload_t{};
                 }
         }
         if constexpr (MASS) {
             if (u - gather0 == room) flush(u);
-            if (col < nh) {
-                f32x4* to = gathered[wave] + (u - gather0) * tile_vecs + (col * TW + NV * grp) / 4;
 #pragma unroll
-                for (int s = 0; s < NS; ++s) to[s] = f32x4{sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]};
+            for (int g = 0; g < NG; ++g)
+                if (col + 16 * g < nh) {
+                    f32x4* to = gathered[wave] + (u - gather0) * tile_vecs + ((col + 16 * g) * TW + NV * grp) / 4;
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) to[s] = f32x4{sc[g][4 * s], sc[g][4 * s + 1], sc[g][4 * s + 2], sc[g][4 * s + 3]};
+                }
+        }
+        float ref[NG], pr[NG][NV];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float mx = sc[g][0];
+#pragma unroll
+            for (int i = 1; i < NV; ++i) mx = fmaxf(mx, sc[g][i]);
+            if (__any(mx > m[g])) {
+                const float mn = fmaxf(m[g], column_all(mx, [](float x, float y) { return fmaxf(x, y); }));
+                const float alpha = m[g] == -INFINITY ? 0.f : ex2(m[g] - mn);
+                m[g] = mn;
+                l[g] *= alpha;
+#pragma unroll
+                for (int n = 0; n < NACC; ++n) acc[g][n] *= alpha;
             }
+            ref[g] = m[g] == -INFINITY ? 0.f : m[g] - OFF;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) { pr[g][i] = ex2(sc[g][i] - ref[g]); sum += pr[g][i]; }
+            l[g] += sum;
         }
-        float mx = sc[0];
-#pragma unroll
-        for (int i = 1; i < NV; ++i) mx = fmaxf(mx, sc[i]);
-        if (__any(mx > m)) {
-            const float mn = fmaxf(m, column_all(mx, [](float x, float y) { return fmaxf(x, y); }));
-            const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
-            m = mn;
-            l *= alpha;
-#pragma unroll
-            for (int n = 0; n < NACC; ++n) acc[n] *= alpha;
-        }
-        const float ref = m == -INFINITY ? 0.f : m - OFF;
-        float pr[NV], sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) { pr[i] = ex2(sc[i] - ref); sum += pr[i]; }
-        l += sum;
         if constexpr (DT == KV_F32) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -436,11 +466,16 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
                 for (int x = 0; x < NX; ++x)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        acc[4 * x + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][x][e]), pr[i], acc[4 * x + e], 0, 0, 0);
+#pragma unroll
+                        for (int g = 0; g < NG; ++g)
+                            acc[g][4 * x + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][x][e]), pr[g][i], acc[g][4 * x + e], 0, 0, 0);
         } else {
-            u32x4 hi, lo;
-            if constexpr (DT == KV_BF16) split8<bf16x8>(pr, &hi, &lo);
-            else split8<f16x8>(pr, &hi, &lo);
+            u32x4 hi[NG], lo[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                if constexpr (DT == KV_BF16) split8<bf16x8>(pr[g], &hi[g], &lo[g]);
+                else split8<f16x8>(pr[g], &hi[g], &lo[g]);
+            }
 #pragma unroll
             for (int x = 0; x < NX; ++x)
 #pragma unroll
@@ -449,21 +484,27 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         v[i] = __builtin_amdgcn_perm(vf[2 * i + 1][x][e >> 1], vf[2 * i][x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-                    acc[x * VEC + e] = Mma<DT>::run(v, hi, acc[x * VEC + e]);
-                    acc[x * VEC + e] = Mma<DT>::run(v, lo, acc[x * VEC + e]);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        acc[g][x * VEC + e] = Mma<DT>::run(v, hi[g], acc[g][x * VEC + e]);
+                        acc[g][x * VEC + e] = Mma<DT>::run(v, lo[g], acc[g][x * VEC + e]);
+                    }
                 }
         }
         if (end) {
-            // component i of accumulator x VEC + e is dim 16 VEC x + (4 grp + i) VEC + e of head col
-            const float L = column_all(l, [](float x, float y) { return x + y; });
-            if (col < nh) {
-                const bool whole = seg0 + cur.nb == u + 1;
-                const int d0 = 4 * grp * VEC;
+            // component i of accumulator x VEC + e is dim 16 VEC x + (4 grp + i) VEC + e of its head
+            const bool whole = seg0 + cur.nb == u + 1;
+            const int d0 = 4 * grp * VEC, slot = 2 * w + (seg0 != u0);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const float L = column_all(l[g], [](float x, float y) { return x + y; });
+                const int c = col + 16 * g;
+                if (c >= nh) continue;
                 if (whole) {
                     // no weight at all (every page bad, or every score -inf): as a row without tokens
                     const float inv = L == 0.f ? 0.f : 1.f / L;
-                    const int64_t head = (int64_t)cur.b * hq + head0_of(cur) + col;
-                    if (grp == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
+                    const int64_t head = (int64_t)cur.b * hq + head0_of(cur) + c;
+                    if (grp == 0) a.lse[head] = L == 0.f ? -INFINITY : ref[g] * LN2 + logf(L);
 #pragma unroll
                     for (int x = 0; x < NX; ++x)
 #pragma unroll
@@ -471,29 +512,25 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
 #pragma unroll
                             for (int e = 0; e < VEC; ++e) {
                                 const int64_t at = head * D + x * 16 * VEC + d0 + i * VEC + e;
-                                const float o = acc[x * VEC + e][i] * inv;
+                                const float o = acc[g][x * VEC + e][i] * inv;
                                 if constexpr (DT == KV_F32) ((float*)a.out)[at] = o;
                                 else if constexpr (DT == KV_BF16) ((bf16_t*)a.out)[at] = (bf16_t)o;
                                 else ((f16_t*)a.out)[at] = (f16_t)o;
                             }
                 } else {
-                    const int slot = 2 * w + (seg0 != u0);
-                    if (grp == 0) a.part_ml[slot * 16 + col] = float2{m == -INFINITY ? -INFINITY : ref, L};
-                    float* po = a.part_out + ((int64_t)slot * a.score_rows + col) * D + d0;
+                    if (grp == 0) a.part_ml[slot * COLS + c] = float2{m[g] == -INFINITY ? -INFINITY : ref[g], L};
+                    float* po = a.part_out + ((int64_t)slot * a.score_rows + c) * D + d0;
 #pragma unroll
                     for (int x = 0; x < NX; ++x)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int e = 0; e < VEC; ++e) po[x * 16 * VEC + i * VEC + e] = acc[x * VEC + e][i];
+                            for (int e = 0; e < VEC; ++e) po[x * 16 * VEC + i * VEC + e] = acc[g][x * VEC + e][i];
                 }
             }
             if (last) break;
             seg0 = u + 1;
-            m = -INFINITY;
-            l = 0.f;
-#pragma unroll
-            for (int n = 0; n < NACC; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+            reset();
         }
         ++u;
         cur = next;
@@ -529,11 +566,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
     constexpr int COLS = D / 4;                      // a lane joins four dims of every ROWS-th part
     constexpr int ROWS = (WAVES ? 64 : 256) / COLS;
     __shared__ f32x4 sums[WAVES ? 1 : ROWS][WAVES ? 1 : COLS];
-    __shared__ float lse2[16];
+    __shared__ float lse2[32];
     __shared__ float2 wave_stat[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cap = tb.max_pages << p.page_shift;
-    const int ngrp = (a.group + 15) >> 4, H = p.heads * ngrp, hq = p.heads * a.group;
+    const int cols = attend_columns(p.dtype, D, a.group), ngrp = (a.group + cols - 1) / cols, H = p.heads * ngrp, hq = p.heads * a.group;
     const bool join = (int)blockIdx.x < joins;
     int b, kvh, h0 = 0, t0 = 0;                      // h0: query head within the group
     if (join) {
@@ -561,9 +598,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
     total = wave_sum(total);
     before = wave_sum(before);
     const Line line(total * H, W);
-    auto parts_of = [&](int grp16) {
+    auto parts_of = [&](int g) {
         Parts q;
-        q.first = before * H + (kvh * ngrp + grp16) * nb;
+        q.first = before * H + (kvh * ngrp + g) * nb;
         q.w0 = line.share_of(q.first);
         q.w1 = line.share_of(q.first + nb - 1);
         return q;
@@ -571,14 +608,14 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
     // {exponent, sum} of head c over parts from, from + step, ...: the caller's lanes together, then the wave's
     auto stats = [&](const Parts& q, int c, int from, int step) {
         float2 x = {-INFINITY, 0.f};
-        for (int w = q.w0 + from; w <= q.w1; w += step) x = stat_join(x, a.part_ml[q.slot(line, w) * 16 + c]);
+        for (int w = q.w0 + from; w <= q.w1; w += step) x = stat_join(x, a.part_ml[q.slot(line, w) * cols + c]);
         for (int o = 32; o; o >>= 1) x = stat_join(x, float2{__shfl_xor(x.x, o), __shfl_xor(x.y, o)});
         return x;
     };
     if (join) {
-        const Parts q = parts_of(h0 >> 4);
+        const Parts q = parts_of(h0 / cols);
         if (q.w0 == q.w1) return;
-        const int c = h0 & 15, n = q.w1 - q.w0 + 1;
+        const int c = h0 % cols, n = q.w1 - q.w0 + 1;
         float2 x = stats(q, c, WAVES ? lane : tid, WAVES ? 64 : 256);
         if (!WAVES) {
             if (lane == 0) wave_stat[wave] = x;
@@ -595,7 +632,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
             for (int j = 0; j < 8; ++j) {
                 const int slot = q.slot(line, q.w0 + min(i + j * ROWS, n - 1));      // (beyond the last part: not added)
                 v[j] = *reinterpret_cast<const f32x4*>(a.part_out + ((int64_t)slot * a.score_rows + c) * D + 4 * d4);
-                f[j] = a.part_ml[slot * 16 + c].x;
+                f[j] = a.part_ml[slot * cols + c].x;
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -631,10 +668,10 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
     const bool whole4 = ((uintptr_t)mass & 15) == 0;
     for (int g = 0; g < ngrp; ++g) {
         const Parts q = parts_of(g);
-        const int nh = min(16, a.group - 16 * g);
+        const int nh = min(cols, a.group - cols * g);
         for (int c = wave; c < nh; c += 4) {
             float x;
-            if (q.w0 == q.w1) x = a.lse[(int64_t)b * hq + kvh * a.group + 16 * g + c] * LOG2E;
+            if (q.w0 == q.w1) x = a.lse[(int64_t)b * hq + kvh * a.group + cols * g + c] * LOG2E;
             else {
                 const float2 st = stats(q, c, lane, 64);
                 x = st.y == 0.f ? -INFINITY : (st.x == -INFINITY ? 0.f : st.x) + __log2f(st.y);
@@ -1122,7 +1159,7 @@ void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hip
 // Tiles of the line if every sequence filled its table.
 static int64_t attend_tiles(const KvPool& p, int B, int group, int max_pages) {
     const int tw = attend_tile(p.dtype);
-    return (((int64_t)max_pages << p.page_shift) + tw - 1) / tw * B * p.heads * ((group + 15) / 16);
+    return (((int64_t)max_pages << p.page_shift) + tw - 1) / tw * B * p.heads * attend_passes(p, group);
 }
 
 bool kv_attend_fits(const KvPool& p, int B, int group, int max_pages) {
@@ -1140,16 +1177,23 @@ static int attend_groups(const KvPool& p, int B, int group, int max_pages) {
 
 // {maximum, sum} and output of two parts per wave (the one it begins with, the one it ends with), and the scores
 size_t kv_attend_ws_bytes(const KvPool& p, int B, int group, int max_pages, bool mass) {
-    const size_t parts = 2 * AT_WAVES * (size_t)attend_groups(p, B, group, max_pages), rows = (size_t)std::min(group, 16);
-    size_t n = parts * 16 * sizeof(float2) + parts * rows * p.dim * sizeof(float);
+    const size_t parts = 2 * AT_WAVES * (size_t)attend_groups(p, B, group, max_pages), cols = (size_t)attend_columns(p, group), rows = std::min((size_t)group, cols);
+    size_t n = parts * cols * sizeof(float2) + parts * rows * p.dim * sizeof(float);
     if (mass) n += (size_t)attend_tiles(p, B, group, max_pages) * rows * attend_tile(p.dtype) * sizeof(float);
     return n;
 }
 
 template <int DT, int D>
 static void attend_launch(const KvPool& p, const KvTable& tb, const KvAttend& a, int W, hipStream_t s) {
-    if (a.mass) kv_attend_kernel<DT, D, true><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
-    else kv_attend_kernel<DT, D, false><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
+    if constexpr (attend_columns(DT, D, 32) == 32) {
+        if (a.group > 16) {
+            if (a.mass) kv_attend_kernel<DT, D, true, 2><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
+            else kv_attend_kernel<DT, D, false, 2><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
+            return;
+        }
+    }
+    if (a.mass) kv_attend_kernel<DT, D, true, 1><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
+    else kv_attend_kernel<DT, D, false, 1><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
 }
 
 template <int D>
@@ -1163,7 +1207,7 @@ static void attend_both(const KvPool& p, const KvTable& tb, const KvAttend& a, i
     // A wave per head where heads are in few parts, on average; a workgroup where they are in many. Longer stretches of mass
     // where there are enough of them to fill the chip. (Workgroups of some 4 us each: their number is what counts.)
     const int64_t heads = (int64_t)tb.B * p.heads * a.group, rows = (int64_t)tb.B * p.heads;
-    const bool waves = waves_all <= 8 * rows * ((a.group + 15) / 16);
+    const bool waves = waves_all <= 8 * rows * attend_passes(p, a.group);
     const int64_t joins = waves ? (heads + 3) / 4 : heads;
     const int mass_tokens = rows * ((cap + 4095) / 4096) >= 512 ? 4096 : 1024;
     const int64_t blocks = joins + (a.mass ? rows * ((cap + mass_tokens - 1) / mass_tokens) : 0);
@@ -1173,9 +1217,9 @@ static void attend_both(const KvPool& p, const KvTable& tb, const KvAttend& a, i
 
 void launch_kv_attend(const KvPool& p, const KvTable& tb, KvAttend a, void* ws, hipStream_t s) {
     const int W = attend_groups(p, tb.B, a.group, tb.max_pages), parts = 2 * W * AT_WAVES;
-    a.score_rows = std::min(a.group, 16);
+    a.score_rows = std::min(a.group, attend_columns(p, a.group));
     a.part_ml = (float2*)ws;
-    a.part_out = (float*)(a.part_ml + (size_t)parts * 16);
+    a.part_out = (float*)(a.part_ml + (size_t)parts * attend_columns(p, a.group));
     a.scores = a.part_out + (size_t)parts * a.score_rows * p.dim;
     if (p.dim == 64) attend_both<64>(p, tb, a, W, s);
     else if (p.dim == 128) attend_both<128>(p, tb, a, W, s);

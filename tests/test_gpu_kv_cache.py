@@ -77,7 +77,7 @@ RAGGED = [0, 1, 7, 8, 9, 31, 32, 33, 63, 64, 65, 127, 128, 129, 130, 300, 0, 515
 
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('d', [64, 128, 256])
-@pytest.mark.parametrize('hkv,group', [(1, 1), (2, 3), (3, 8), (1, 16), (2, 17), (1, 40)])
+@pytest.mark.parametrize('hkv,group', [(1, 1), (2, 3), (3, 8), (1, 16), (2, 17), (1, 32), (1, 33), (1, 40)])
 def test_attend_ragged(dtype, d, hkv, group):
     page = {1: 8, 2: 16, 3: 64}[hkv]
     cache, table, lengths = _make(d + group, RAGGED, hkv, d, page, dtype)
