@@ -311,7 +311,7 @@ typedef struct TacoKvPool {
  *   positions [B, kv_heads, side_ld] int32, or NULL: first[b] + t (first NULL = starts) for the new slots
  *   lengths_out [B] int32: starts[b] + counts[b]
  * side_ld >= max_pages * page_size. Tokens beyond the table's capacity are dropped (TACO_KV_BAD_LENGTH). The pages that
- * are written must be the sequence's own. */
+ * are written must be the sequence's own, and k and v no part of the pool. */
 int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
                    const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
                    const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride, int32_t T,
@@ -324,7 +324,9 @@ int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_l
  * q [B, q_heads, head_dim] by strides of batch and head, q_heads = group * kv_heads; out [B, q_heads, head_dim] and
  * lse [B, q_heads] (fp32, natural log) contiguous; mass [B, kv_heads, side_ld] fp32. Pages may be shared between
  * sequences. A row without tokens, or whose scores are all -inf, gives out 0 and lse -inf and leaves its mass alone.
- * What masked slots and unused pages hold (NaN, infinities) has no influence. Sums and softmax statistics are fp32. */
+ * What masked slots and unused pages hold (NaN, infinities) has no influence; a NaN or an infinity among a row's own tokens
+ * makes that row's output NaN or infinite and no other. Sums and softmax statistics are fp32. The same call gives the same
+ * bits; how a row's sums are cut depends on all lengths of the call, so a row's last bits may differ in another batch. */
 size_t taco_kv_attend_workspace_bytes(const TacoKvPool* pool, int32_t B, int32_t q_heads, int32_t max_pages,
                                       int32_t with_mass);
 int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,

@@ -245,6 +245,10 @@ struct Cursor {
     int nb, len;                         // tiles and tokens of the sequence
 };
 
+// What it reaches, with the weights collected: 32 sequences of up to 32768 tokens (655 k in all), 32 heads over 8 of 128, bf16,
+// pages of 32: 405 us for 2.65 GB of K and V, 6.5 TB/s (and 84 MB of scores written); without the weights 32 x 16384 tokens
+// 6.4 / 6.85 / 6.7 TB/s at pages of 16 / 32 / 128, 5.8 where a page keeps its heads side by side. A plain read of as many
+// bytes in order reaches 7.0 to 7.4. A call of nothing much takes 8 us here, five loads one after the other.
 template <int DT, int D, bool MASS, int NG>
 __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
     using S = AttendShape<DT, D>;
@@ -558,13 +562,14 @@ __device__ __forceinline__ float2 stat_join(float2 x, float2 y) {
 // do mass_tokens tokens (a multiple of 1024) of mass[b][h] += sum over the query heads of h of exp(score - lse) each, from
 // the scores that kv_attend_kernel left. The lse of a head in parts is computed by whoever needs it (a few values), so
 // that both fit one launch. Short work that waits for one dependent load after the other, so every step loads all it needs
-// at once: a part's {exponent, sum} per lane, eight rows of the parts' outputs per lane, four tokens of a head's
-// scores per lane.
+// at once: a part's {exponent, sum} per lane, eight or sixteen rows of the parts' outputs per lane, four tokens of a head's
+// scores per lane. (5 us where there is little to do; 36 us for the 126 MB of scores and masses of 32 sequences up to 32768.)
 template <int D, bool WAVES>
 __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTable tb, const KvAttend a, int W, int tw, int joins,
                                                       int mass_tokens) {
     constexpr int COLS = D / 4;                      // a lane joins four dims of every ROWS-th part
     constexpr int ROWS = (WAVES ? 64 : 256) / COLS;
+    constexpr int AHEAD = WAVES ? 8 : 16;            // parts a lane loads at once
     __shared__ f32x4 sums[WAVES ? 1 : ROWS][WAVES ? 1 : COLS];
     __shared__ float lse2[32];
     __shared__ float2 wave_stat[4];
@@ -625,17 +630,17 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         const float ref = x.x == -INFINITY ? 0.f : x.x, L = x.y;
         const int id = WAVES ? lane : tid, d4 = id % COLS, k = id / COLS;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int i = k; i < n; i += 8 * ROWS) {
-            f32x4 v[8];
-            float f[8];
+        for (int i = k; i < n; i += AHEAD * ROWS) {
+            f32x4 v[AHEAD];
+            float f[AHEAD];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < AHEAD; ++j) {
                 const int slot = q.slot(line, q.w0 + min(i + j * ROWS, n - 1));      // (beyond the last part: not added)
                 v[j] = *reinterpret_cast<const f32x4*>(a.part_out + ((int64_t)slot * a.score_rows + c) * D + 4 * d4);
                 f[j] = a.part_ml[slot * cols + c].x;
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < AHEAD; ++j)
                 if (i + j * ROWS < n) o += v[j] * ex2(f[j] - ref);
         }
         if constexpr (WAVES) {
@@ -719,7 +724,7 @@ struct SelectShared {
     uint32_t list[EV_LIST];
     int wave_a[EV_WAVES], wave_b[EV_WAVES];
     uint32_t digit;
-    int left, same, listed, newest, kept_low;        // same: keys with the digit
+    int left, same, listed, newest;                  // same: keys with the digit
 };
 
 // One (sequence, kv head) as the select kernels see it.
@@ -1004,7 +1009,7 @@ __device__ __forceinline__ void move_rows(const KvPool& p, const KvTable& tb, co
 
 // One workgroup per (sequence, kv head). The n-th greatest key by a radix select of 11 + 11 + 10 bits, then one pass in
 // slot order. Masses and positions stay in registers, so they are read once, together; what is left are LDS counters and a
-// dozen barriers.
+// dozen barriers, which bound it: 10 us at 2049 tokens, 15 at 8192, a head to a CU.
 template <bool MOVE>
 __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, const KvTable tb, const KvEvict a) {
     __shared__ SelectShared sh;
@@ -1024,7 +1029,8 @@ __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, c
 // The same for tables of more slots than a workgroup holds: a workgroup per chunk, four launches. Each workgroup works out
 // the head's threshold for itself from what the one before left: the chunks' newest positions, the chunks' histograms of the
 // first digit, the chunks' lists of the keys that share the threshold's first digit. Sums over chunks before
-// its own give it the ranks of its slots, so nothing waits for anything and no counter is shared.
+// its own give it the ranks of its slots, so nothing waits for anything and no counter is shared. (32 heads of 65536 tokens:
+// 5 + 5 + 9 + 19 us.)
 struct ChunkWork {
     int32_t* newest;                     // [chunks]
     uint32_t* hist;                      // [chunks][2048]
@@ -1207,7 +1213,7 @@ static void attend_both(const KvPool& p, const KvTable& tb, const KvAttend& a, i
     // A wave per head where heads are in few parts, on average; a workgroup where they are in many. Longer stretches of mass
     // where there are enough of them to fill the chip. (Workgroups of some 4 us each: their number is what counts.)
     const int64_t heads = (int64_t)tb.B * p.heads * a.group, rows = (int64_t)tb.B * p.heads;
-    const bool waves = waves_all <= 8 * rows * attend_passes(p, a.group);
+    const bool waves = waves_all <= 16 * rows * attend_passes(p, a.group);
     const int64_t joins = waves ? (heads + 3) / 4 : heads;
     const int mass_tokens = rows * ((cap + 4095) / 4096) >= 512 ? 4096 : 1024;
     const int64_t blocks = joins + (a.mass ? rows * ((cap + mass_tokens - 1) / mass_tokens) : 0);

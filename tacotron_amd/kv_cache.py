@@ -8,7 +8,8 @@ collected `mass` being the alignments summed over the steps.
 The cache object holds the pool's geometry and a status word. Everything else - page tables, lengths, masses, positions -
 is the caller's and is passed to each call, so one pool serves any number of batches and a captured HIP graph follows what
 the tensors hold when it runs. Calls are queued on torch's current stream of the pool's device and synchronise nothing;
-workspaces and results come from torch's allocator, so calls on several streams do not share any."""
+workspaces and results come from torch's allocator, so calls on several streams do not share any. A serving form: no
+gradients are recorded."""
 import ctypes
 import math
 
@@ -64,8 +65,9 @@ class KvCache:
         return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
 
     def status(self):
-        """Synchronises; raises TacoError if any call since the last status() met a length outside its table's capacity
-        or a page id outside the pool (which it treated as masked)."""
+        """Synchronises the device; raises TacoError if any call since the last status() met a length outside its table's
+        capacity or a page id outside the pool (which it treated as masked)."""
+        torch.cuda.synchronize(self.device)
         bits = int(self._status.item())
         if bits:
             self._status.zero_()
@@ -124,6 +126,7 @@ class KvCache:
         return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
     def _stream(self):
+        # the handle alone: torch.cuda.current_stream builds an object around it
         return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     # ---- the operators
