@@ -239,140 +239,40 @@ __device__ __forceinline__ void split8(const float* p, u32x4* hi, u32x4* lo) {
     *lo = __builtin_bit_cast(u32x4, l);
 }
 
-// A tile of the line.
-struct Cursor {
-    int b, hg, tile;                     // sequence, head group, tile of its tokens
-    int nb, len;                         // tiles and tokens of the sequence
-};
-
-// What it reaches, with the weights collected: 32 sequences of up to 32768 tokens (655 k in all), 32 heads over 8 of 128, bf16,
-// pages of 32: 405 us for 2.65 GB of K and V, 6.5 TB/s (and 84 MB of scores written); without the weights 32 x 16384 tokens
-// 6.4 / 6.85 / 6.7 TB/s at pages of 16 / 32 / 128, 5.8 where a page keeps its heads side by side. A plain read of as many
-// bytes in order reaches 7.0 to 7.4. A call of nothing much takes 8 us here, five loads one after the other.
-template <int DT, int D, bool MASS, int NG>
-__global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
+// What a wave holds of one head group and tile, and the steps of a tile. NG 16-wide tiles of heads: a lane has heads
+// col + 16 g of the group's stretch, g < NG.
+template <int DT, int D, int NG>
+struct AttendWave {
     using S = AttendShape<DT, D>;
-    constexpr int TW = S::TW, VEC = S::VEC, NX = S::NX, NACC = S::NACC, KL = S::KL, ES = S::ES;
-    constexpr int NS = TW / 16, NV = TW / 4;         // 16-token blocks; tokens a lane holds, NV (lane >> 4) and on
-    constexpr int COLS = 16 * NG;                    // a lane has heads col + 16 g of the group's stretch, g < NG
+    static constexpr int TW = S::TW, VEC = S::VEC, NX = S::NX, NACC = S::NACC, KL = S::KL, ES = S::ES;
+    static constexpr int NS = TW / 16, NV = TW / 4;  // 16-token blocks; tokens a lane holds, NV (lane >> 4) and on
+    static constexpr int COLS = 16 * NG;
     // fp16 weights are kept 2^14 too large (the sums with them): at most 16384, and 2^-28 is still a normal number, so that
     // many small weights beside a large one are not lost
-    constexpr float OFF = DT == KV_F16 ? 14.f : 0.f;
+    static constexpr float OFF = DT == KV_F16 ? 14.f : 0.f;
     typedef typename std::conditional<VEC * ES == 16, u32x4, u32x2>::type vload_t;
-    __shared__ f32x4 gathered[MASS ? AT_WAVES : 1][MASS ? S::GATHER / 16 : 1];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int col = lane & 15, grp = lane >> 4;
-    const int ktok = NS == 2 ? 8 * (col >> 2) + (col & 3) : col;     // token of this lane's K row, block 0
-    const int cap = tb.max_pages << p.page_shift, w = blockIdx.x * AT_WAVES + wave;
-    const int ngrp = (a.group + COLS - 1) / COLS, H = p.heads * ngrp, hq = p.heads * a.group;
-
-    // the line, from the tiles of the first 64 sequences (a lane each; their lengths stay at hand) and, 64 by 64, the rest
-    auto tiles = [](int len) { return (len + TW - 1) / TW; };
-    const int raw64 = lane < tb.B ? a.lengths[lane] : 0, len64 = max(0, min(raw64, cap));
-    auto len_of = [&](int b) { return b < 64 ? __builtin_amdgcn_readlane(len64, b) : __builtin_amdgcn_readfirstlane(max(0, min(a.lengths[b], cap))); };
-    const int first64 = tiles(len64), scan64 = wave_scan(first64);
-    int total = __builtin_amdgcn_readlane(scan64, 63);
-    if (tb.B > 64) {
-        int more = 0;
-        for (int i = lane + 64; i < tb.B; i += 64) more += tiles_of(tb, a.lengths, i, cap, TW);
-        total += wave_sum(more);
-    }
-    const Line line(total * H, gridDim.x * AT_WAVES);
-    const int u0 = line.begin(w), u1 = line.begin(w + 1);
-
-    // the check of the lengths, and sequences without tokens
-    if (w == 0 && len64 != raw64) atomicOr(p.status, KV_BAD_LENGTH);
-    for (int b = w; b < tb.B; b += gridDim.x * AT_WAVES) {
-        if (b >= 64) (void)clamp_len(a.lengths[b], cap, p.status, lane == 0);
-        if (len_of(b)) continue;
-        for (int i = lane; i < hq * D * ES / 4; i += 64) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
-        for (int i = lane; i < hq; i += 64) a.lse[(int64_t)b * hq + i] = -INFINITY;
-    }
-    if (u0 == u1) return;
-
-    int b0 = 0, before = 0;                          // the sequence of tile u0, and the tiles before it
-    for (int x = first64, inc = scan64;;) {
-        const unsigned long long hit = __ballot(before + inc * H > u0);
-        if (hit) {
-            const int at = __ffsll(hit) - 1;
-            b0 += at;
-            before += __builtin_amdgcn_readlane(inc - x, at) * H;
-            break;
-        }
-        before += __builtin_amdgcn_readlane(inc, 63) * H;
-        b0 += 64;
-        x = b0 + lane < tb.B ? tiles_of(tb, a.lengths, b0 + lane, cap, TW) : 0;
-        inc = wave_scan(x);
-    }
-    auto at_sequence = [&](Cursor& c) {
-        c.len = len_of(c.b);
-        c.nb = tiles(c.len);
-    };
-    // (called for tiles of the share only, so there is a next one)
-    auto advance = [&](Cursor c) {
-        if (++c.tile == c.nb) {
-            c.tile = 0;
-            if (++c.hg == H) {
-                c.hg = 0;
-                do {
-                    ++c.b;
-                    at_sequence(c);
-                } while (c.nb == 0);
-            }
-        }
-        return c;
-    };
-    Cursor cur;
-    cur.b = __builtin_amdgcn_readfirstlane(b0);
-    at_sequence(cur);
-    cur.hg = (u0 - before) / cur.nb;
-    cur.tile = (u0 - before) % cur.nb;
-
-    // Page of slot t of a cursor's sequence; of its last one where t lies behind it, so that every row below is in the pool
-    // (and of page 0 where the id is bad): what is masked is read and thrown away. A lane's NV tokens share a page.
-    auto page_of = [&](const Cursor& c, int t) { return tb.table[(int64_t)c.b * tb.ld + (min(c.tile * TW + t, c.len - 1) >> p.page_shift)]; };
-    auto bad_id = [&](int page) { return (unsigned)page >= (unsigned)p.num_pages; };
-    const int mask = p.page_size - 1;
+    const KvPool& p;
+    const KvTable& tb;
+    const KvAttend& a;
+    int lane, col, grp, ktok;                        // ktok: token of this lane's K row, block 0
+    int ngrp, hq;
     u32x4 kf[NS][KL], qf[NG][KL];
-    auto load_k = [&](const Cursor& c, int page) {
-        const int kvh = c.hg / ngrp;
-        const char* r = (const char*)p.k + ((int64_t)kvh * p.k_st[1] + (int64_t)(bad_id(page) ? 0 : page) * p.k_st[0] +
-                                            (int64_t)((c.tile * TW + ktok) & mask) * p.k_st[2]) * ES + grp * 16;
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int j = 0; j < KL; ++j)
-                kf[s][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(r + 4 * s * p.k_st[2] * ES + j * 64));
-    };
-    auto head0_of = [&](const Cursor& c) { return c.hg / ngrp * a.group + c.hg % ngrp * COLS; };
-    auto heads_of = [&](const Cursor& c) { return min(COLS, a.group - c.hg % ngrp * COLS); };
-    auto load_q = [&](const Cursor& c) {
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const int head = head0_of(c) + min(col + 16 * g, heads_of(c) - 1);      // (idle columns: the last head again)
-            const char* q = (const char*)a.q + ((int64_t)c.b * a.q_st[0] + (int64_t)head * a.q_st[1]) * ES + grp * 16;
-#pragma unroll
-            for (int j = 0; j < KL; ++j) qf[g][j] = *reinterpret_cast<const u32x4*>(q + j * 64);
-        }
-    };
+    vload_t vf[NV][NX];
+    float sc[NG][NV];                                // scores of the lane's tokens, in units of ln 2
+    float m[NG], l[NG], ref[NG];                     // maximum (column-wide), sum (this lane's), exponent the sums refer to
+    f32x4 acc[NG][NACC];                             // component i of x VEC + e: dim 16 VEC x + (4 grp + i) VEC + e
 
-    // Scores for the weights of `mass`: [tile][score_rows][TW]. A wave gathers those of tiles gather0, gather0 + 1, ... and
-    // writes them out when there is room for no more, and at the end: a trickle of writes among the reads costs far more of
-    // the memory's time than their bytes.
-    const int tile_vecs = a.score_rows * TW / 4, room = S::GATHER / 16 / tile_vecs;
-    int gather0 = u0;
-    auto flush = [&](int upto) {
-        f32x4* to = (f32x4*)a.scores + (int64_t)gather0 * tile_vecs;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int j = lane; j < (upto - gather0) * tile_vecs; j += 64) to[j] = gathered[wave][j];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        gather0 = upto;
-    };
-
-    float m[NG], l[NG];
-    f32x4 acc[NG][NACC];
-    auto reset = [&]() INLINE {
+    __device__ __forceinline__ AttendWave(const KvPool& p_, const KvTable& tb_, const KvAttend& a_) : p(p_), tb(tb_), a(a_) {
+        lane = threadIdx.x & 63;
+        col = lane & 15;
+        grp = lane >> 4;
+        ktok = NS == 2 ? 8 * (col >> 2) + (col & 3) : col;
+        ngrp = (a.group + COLS - 1) / COLS;
+        hq = p.heads * a.group;
+        reset();
+    }
+    __device__ __forceinline__ void reset() {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             m[g] = -INFINITY;
@@ -380,31 +280,46 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
 #pragma unroll
             for (int n = 0; n < NACC; ++n) acc[g][n] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-    };
-    reset();
-    int vpage = page_of(cur, NV * grp);
-    load_q(cur);
-    load_k(cur, page_of(cur, ktok));
-    Cursor next = u0 + 1 < u1 ? advance(cur) : cur;
-    int kpage1 = page_of(next, ktok), vpage1 = page_of(next, NV * grp);
-    int seg0 = u0;                                   // where this wave began with the head
+    }
+    __device__ __forceinline__ int head0(int hg) const { return hg / ngrp * a.group + hg % ngrp * COLS; }
+    __device__ __forceinline__ int heads(int hg) const { return min(COLS, a.group - hg % ngrp * COLS); }
 
-    for (int u = u0;;) {
-        // pages of the tile after the next, then V of this one: in flight during the first product
-        const bool last = u + 1 == u1;
-        const Cursor next2 = u + 2 < u1 ? advance(next) : next;
-        const int kpage2 = page_of(next2, ktok), vpage2 = page_of(next2, NV * grp);
-        const int t = cur.tile * TW, tok = t + NV * grp;
-        const bool bad = bad_id(vpage);
-        vload_t vf[NV][NX];
-        const char* r = (const char*)p.v + ((int64_t)(cur.hg / ngrp) * p.v_st[1] + (int64_t)(bad ? 0 : vpage) * p.v_st[0] +
-                                            (int64_t)(tok & mask) * p.v_st[2]) * ES + col * VEC * ES;
+    // Page of slot t of sequence b; of its last one where t lies behind it, so that every row below is in the pool (and of page
+    // 0 where the id is bad): what is masked is read and thrown away. A lane's NV tokens share a page.
+    __device__ __forceinline__ int page_of(int b, int len, int t) const { return tb.table[(int64_t)b * tb.ld + (min(t, len - 1) >> p.page_shift)]; }
+    __device__ __forceinline__ bool bad_id(int page) const { return (unsigned)page >= (unsigned)p.num_pages; }
+    __device__ __forceinline__ int k_page(int b, int len, int t) const { return page_of(b, len, t + ktok); }
+    __device__ __forceinline__ int v_page(int b, int len, int t) const { return page_of(b, len, t + NV * grp); }
+
+    __device__ __forceinline__ void load_q(int b, int hg) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const int head = head0(hg) + min(col + 16 * g, heads(hg) - 1);      // (idle columns: the last head again)
+            const char* q = (const char*)a.q + ((int64_t)b * a.q_st[0] + (int64_t)head * a.q_st[1]) * ES + grp * 16;
+#pragma unroll
+            for (int j = 0; j < KL; ++j) qf[g][j] = *reinterpret_cast<const u32x4*>(q + j * 64);
+        }
+    }
+    // K and V rows of the tile at t. (Past the caches: read once.)
+    __device__ __forceinline__ void load_k(int hg, int t, int page) {
+        const char* r = (const char*)p.k + ((int64_t)(hg / ngrp) * p.k_st[1] + (int64_t)(bad_id(page) ? 0 : page) * p.k_st[0] +
+                                            (int64_t)((t + ktok) & (p.page_size - 1)) * p.k_st[2]) * ES + grp * 16;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < KL; ++j)
+                kf[s][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(r + 4 * s * p.k_st[2] * ES + j * 64));
+    }
+    __device__ __forceinline__ void load_v(int hg, int t, int page) {
+        const char* r = (const char*)p.v + ((int64_t)(hg / ngrp) * p.v_st[1] + (int64_t)(bad_id(page) ? 0 : page) * p.v_st[0] +
+                                            (int64_t)((t + NV * grp) & (p.page_size - 1)) * p.v_st[2]) * ES + col * VEC * ES;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int x = 0; x < NX; ++x)
                 vf[i][x] = __builtin_nontemporal_load(reinterpret_cast<const vload_t*>(r + i * p.v_st[2] * ES + x * 16 * VEC * ES));
-        float sc[NG][NV];
+    }
+    __device__ __forceinline__ void scores() {
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -415,35 +330,29 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sc[g][4 * s + i] = c[i] * a.scale2;
             }
-        const bool end = last || next.tile == 0;     // of the head, as far as it is this wave's
-        const int nh = heads_of(cur);
-        if (!last) {
-            if (end) load_q(next);
-            load_k(next, kpage1);
-        }
-        if (t + TW > cur.len || __any(bad)) {
-            // masked slots: score -inf, and no row that 0 could be multiplied with to give NaN
-            if (bad && tok < cur.len) atomicOr(p.status, KV_BAD_PAGE);
+    }
+    // Slots behind the length or of a bad page: score -inf, and no row that 0 could be multiplied with to give NaN.
+    __device__ __forceinline__ void mask(int len, int t, int page) {
+        const int tok = t + NV * grp;
+        const bool bad = bad_id(page);
+        if (t + TW <= len && !__any(bad)) return;
+        if (bad && tok < len) atomicOr(p.status, KV_BAD_PAGE);
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (bad || tok + i >= cur.len) {
+        for (int i = 0; i < NV; ++i)
+            if (bad || tok + i >= len) {
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) sc[g][i] = -INFINITY;
+                for (int g = 0; g < NG; ++g) sc[g][i] = -INFINITY;
 #pragma unroll
-                    for (int x = 0; x < NX; ++x) vf[i][x] = vload_t{};
-                }
-        }
-        if constexpr (MASS) {
-            if (u - gather0 == room) flush(u);
+                for (int x = 0; x < NX; ++x) vf[i][x] = vload_t{};
+            }
+    }
+    // The lane's scores of head tile g as they go into a [head][TW] table.
+    __device__ __forceinline__ void put_scores(int g, f32x4* to) const {
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
-                if (col + 16 * g < nh) {
-                    f32x4* to = gathered[wave] + (u - gather0) * tile_vecs + ((col + 16 * g) * TW + NV * grp) / 4;
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) to[s] = f32x4{sc[g][4 * s], sc[g][4 * s + 1], sc[g][4 * s + 2], sc[g][4 * s + 3]};
-                }
-        }
-        float ref[NG], pr[NG][NV];
+        for (int s = 0; s < NS; ++s) to[s] = f32x4{sc[g][4 * s], sc[g][4 * s + 1], sc[g][4 * s + 2], sc[g][4 * s + 3]};
+    }
+    __device__ __forceinline__ void accumulate() {
+        float pr[NG][NV];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             float mx = sc[g][0];
@@ -495,46 +404,179 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
                     }
                 }
         }
+    }
+    __device__ __forceinline__ float sum_of(int g) const { return column_all(l[g], [](float x, float y) { return x + y; }); }
+    __device__ __forceinline__ float exponent_of(int g) const { return m[g] == -INFINITY ? -INFINITY : m[g] - OFF; }
+};
+
+template <int DT>
+__device__ __forceinline__ void store_out(void* out, int64_t at, float x) {
+    if constexpr (DT == KV_F32) ((float*)out)[at] = x;
+    else if constexpr (DT == KV_BF16) ((bf16_t*)out)[at] = (bf16_t)x;
+    else ((f16_t*)out)[at] = (f16_t)x;
+}
+
+// A tile of the line.
+struct Cursor {
+    int b, hg, tile;                     // sequence, head group, tile of its tokens
+    int nb, len;                         // tiles and tokens of the sequence
+};
+
+// What it reaches, with the weights collected: 32 sequences of up to 32768 tokens (655 k in all), 32 heads over 8 of 128, bf16,
+// pages of 32: 405 us for 2.65 GB of K and V, 6.5 TB/s (and 84 MB of scores written); without the weights 32 x 16384 tokens
+// 6.4 / 6.85 / 6.7 TB/s at pages of 16 / 32 / 128, 5.8 where a page keeps its heads side by side. A plain read of as many
+// bytes in order reaches 7.0 to 7.4. A call of nothing much takes 8 us here, five loads one after the other.
+template <int DT, int D, bool MASS, int NG>
+__global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
+    using S = AttendShape<DT, D>;
+    using Wave = AttendWave<DT, D, NG>;
+    constexpr int TW = S::TW, VEC = S::VEC, NX = S::NX, ES = S::ES, COLS = Wave::COLS;
+    __shared__ f32x4 gathered[MASS ? AT_WAVES : 1][MASS ? S::GATHER / 16 : 1];
+    Wave x(p, tb, a);
+    const int lane = x.lane, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cap = tb.max_pages << p.page_shift, w = blockIdx.x * AT_WAVES + wave;
+    const int H = p.heads * x.ngrp, hq = x.hq;
+
+    // the line, from the tiles of the first 64 sequences (a lane each; their lengths stay at hand) and, 64 by 64, the rest
+    auto tiles = [](int len) { return (len + TW - 1) / TW; };
+    const int raw64 = lane < tb.B ? a.lengths[lane] : 0, len64 = max(0, min(raw64, cap));
+    auto len_of = [&](int b) INLINE { return b < 64 ? __builtin_amdgcn_readlane(len64, b) : __builtin_amdgcn_readfirstlane(max(0, min(a.lengths[b], cap))); };
+    const int first64 = tiles(len64), scan64 = wave_scan(first64);
+    int total = __builtin_amdgcn_readlane(scan64, 63);
+    if (tb.B > 64) {
+        int more = 0;
+        for (int i = lane + 64; i < tb.B; i += 64) more += tiles_of(tb, a.lengths, i, cap, TW);
+        total += wave_sum(more);
+    }
+    const Line line(total * H, gridDim.x * AT_WAVES);
+    const int u0 = line.begin(w), u1 = line.begin(w + 1);
+
+    // the check of the lengths, and sequences without tokens
+    if (w == 0 && len64 != raw64) atomicOr(p.status, KV_BAD_LENGTH);
+    for (int b = w; b < tb.B; b += gridDim.x * AT_WAVES) {
+        if (b >= 64) (void)clamp_len(a.lengths[b], cap, p.status, lane == 0);
+        if (len_of(b)) continue;
+        for (int i = lane; i < hq * D * ES / 4; i += 64) ((uint32_t*)a.out)[(int64_t)b * (hq * D * ES / 4) + i] = 0;
+        for (int i = lane; i < hq; i += 64) a.lse[(int64_t)b * hq + i] = -INFINITY;
+    }
+    if (u0 == u1) return;
+
+    int b0 = 0, before = 0;                          // the sequence of tile u0, and the tiles before it
+    for (int n = first64, inc = scan64;;) {
+        const unsigned long long hit = __ballot(before + inc * H > u0);
+        if (hit) {
+            const int at = __ffsll(hit) - 1;
+            b0 += at;
+            before += __builtin_amdgcn_readlane(inc - n, at) * H;
+            break;
+        }
+        before += __builtin_amdgcn_readlane(inc, 63) * H;
+        b0 += 64;
+        n = b0 + lane < tb.B ? tiles_of(tb, a.lengths, b0 + lane, cap, TW) : 0;
+        inc = wave_scan(n);
+    }
+    auto at_sequence = [&](Cursor& c) INLINE {
+        c.len = len_of(c.b);
+        c.nb = tiles(c.len);
+    };
+    // (called for tiles of the share only, so there is a next one)
+    auto advance = [&](Cursor c) INLINE {
+        if (++c.tile == c.nb) {
+            c.tile = 0;
+            if (++c.hg == H) {
+                c.hg = 0;
+                do {
+                    ++c.b;
+                    at_sequence(c);
+                } while (c.nb == 0);
+            }
+        }
+        return c;
+    };
+    Cursor cur;
+    cur.b = __builtin_amdgcn_readfirstlane(b0);
+    at_sequence(cur);
+    cur.hg = (u0 - before) / cur.nb;
+    cur.tile = (u0 - before) % cur.nb;
+    auto k_page = [&](const Cursor& c) INLINE { return x.k_page(c.b, c.len, c.tile * TW); };
+    auto v_page = [&](const Cursor& c) INLINE { return x.v_page(c.b, c.len, c.tile * TW); };
+
+    // Scores for the weights of `mass`: [tile][score_rows][TW]. A wave gathers those of tiles gather0, gather0 + 1, ... and
+    // writes them out when there is room for no more, and at the end: a trickle of writes among the reads costs far more of
+    // the memory's time than their bytes.
+    const int tile_vecs = a.score_rows * TW / 4, room = S::GATHER / 16 / tile_vecs;
+    int gather0 = u0;
+    auto flush = [&](int upto) INLINE {
+        f32x4* to = (f32x4*)a.scores + (int64_t)gather0 * tile_vecs;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int j = lane; j < (upto - gather0) * tile_vecs; j += 64) to[j] = gathered[wave][j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        gather0 = upto;
+    };
+
+    int vpage = v_page(cur);
+    x.load_q(cur.b, cur.hg);
+    x.load_k(cur.hg, cur.tile * TW, k_page(cur));
+    Cursor next = u0 + 1 < u1 ? advance(cur) : cur;
+    int kpage1 = k_page(next), vpage1 = v_page(next);
+    int seg0 = u0;                                   // where this wave began with the head
+
+    for (int u = u0;;) {
+        // pages of the tile after the next, then V of this one: in flight during the first product
+        const bool last = u + 1 == u1;
+        const Cursor next2 = u + 2 < u1 ? advance(next) : next;
+        const int kpage2 = k_page(next2), vpage2 = v_page(next2);
+        x.load_v(cur.hg, cur.tile * TW, vpage);
+        x.scores();
+        const bool end = last || next.tile == 0;     // of the head, as far as it is this wave's
+        const int nh = x.heads(cur.hg);
+        if (!last) {
+            if (end) x.load_q(next.b, next.hg);
+            x.load_k(next.hg, next.tile * TW, kpage1);
+        }
+        x.mask(cur.len, cur.tile * TW, vpage);
+        if constexpr (MASS) {
+            if (u - gather0 == room) flush(u);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                if (x.col + 16 * g < nh)
+                    x.put_scores(g, gathered[wave] + (u - gather0) * tile_vecs + ((x.col + 16 * g) * TW + Wave::NV * x.grp) / 4);
+        }
+        x.accumulate();
         if (end) {
-            // component i of accumulator x VEC + e is dim 16 VEC x + (4 grp + i) VEC + e of its head
             const bool whole = seg0 + cur.nb == u + 1;
-            const int d0 = 4 * grp * VEC, slot = 2 * w + (seg0 != u0);
+            const int d0 = 4 * x.grp * VEC, slot = 2 * w + (seg0 != u0);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float L = column_all(l[g], [](float x, float y) { return x + y; });
-                const int c = col + 16 * g;
+                const float L = x.sum_of(g);
+                const int c = x.col + 16 * g;
                 if (c >= nh) continue;
                 if (whole) {
                     // no weight at all (every page bad, or every score -inf): as a row without tokens
                     const float inv = L == 0.f ? 0.f : 1.f / L;
-                    const int64_t head = (int64_t)cur.b * hq + head0_of(cur) + c;
-                    if (grp == 0) a.lse[head] = L == 0.f ? -INFINITY : ref[g] * LN2 + logf(L);
+                    const int64_t head = (int64_t)cur.b * hq + x.head0(cur.hg) + c;
+                    if (x.grp == 0) a.lse[head] = L == 0.f ? -INFINITY : x.ref[g] * LN2 + logf(L);
 #pragma unroll
-                    for (int x = 0; x < NX; ++x)
+                    for (int n = 0; n < NX; ++n)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int e = 0; e < VEC; ++e) {
-                                const int64_t at = head * D + x * 16 * VEC + d0 + i * VEC + e;
-                                const float o = acc[g][x * VEC + e][i] * inv;
-                                if constexpr (DT == KV_F32) ((float*)a.out)[at] = o;
-                                else if constexpr (DT == KV_BF16) ((bf16_t*)a.out)[at] = (bf16_t)o;
-                                else ((f16_t*)a.out)[at] = (f16_t)o;
-                            }
+                            for (int e = 0; e < VEC; ++e)
+                                store_out<DT>(a.out, head * D + n * 16 * VEC + d0 + i * VEC + e, x.acc[g][n * VEC + e][i] * inv);
                 } else {
-                    if (grp == 0) a.part_ml[slot * COLS + c] = float2{m[g] == -INFINITY ? -INFINITY : ref[g], L};
+                    if (x.grp == 0) a.part_ml[slot * COLS + c] = float2{x.exponent_of(g), L};
                     float* po = a.part_out + ((int64_t)slot * a.score_rows + c) * D + d0;
 #pragma unroll
-                    for (int x = 0; x < NX; ++x)
+                    for (int n = 0; n < NX; ++n)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int e = 0; e < VEC; ++e) po[x * 16 * VEC + i * VEC + e] = acc[g][x * VEC + e][i];
+                            for (int e = 0; e < VEC; ++e) po[n * 16 * VEC + i * VEC + e] = x.acc[g][n * VEC + e][i];
                 }
             }
             if (last) break;
             seg0 = u + 1;
-            reset();
+            x.reset();
         }
         ++u;
         cur = next;
