@@ -326,7 +326,8 @@ int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_l
  * sequences. A row without tokens, or whose scores are all -inf, gives out 0 and lse -inf and leaves its mass alone.
  * What masked slots and unused pages hold (NaN, infinities) has no influence; a NaN or an infinity among a row's own tokens
  * makes that row's output NaN or infinite and no other. Sums and softmax statistics are fp32. The same call gives the same
- * bits; how a row's sums are cut depends on all lengths of the call, so a row's last bits may differ in another batch. */
+ * bits; how a row's sums are cut depends on the batch and all its lengths, so a row's last bits may differ in another. Short
+ * memories need no workspace; the size is then given as the least there is, 16 bytes. */
 size_t taco_kv_attend_workspace_bytes(const TacoKvPool* pool, int32_t B, int32_t q_heads, int32_t max_pages,
                                       int32_t with_mass);
 int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,

@@ -25,6 +25,9 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }   // (flushes results below 2^-126)
 
+// log of sum 2^ref, the same bits wherever it is computed.
+__device__ __forceinline__ float log_sum(float ref, float sum) { return __builtin_fmaf(ref, LN2, logf(sum)); }
+
 __device__ __forceinline__ int clamp_len(int n, int cap, int32_t* status, bool report) {
     if (n >= 0 && n <= cap) return n;
     if (report) atomicOr(status, KV_BAD_LENGTH);
@@ -555,7 +558,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
                     // no weight at all (every page bad, or every score -inf): as a row without tokens
                     const float inv = L == 0.f ? 0.f : 1.f / L;
                     const int64_t head = (int64_t)cur.b * hq + x.head0(cur.hg) + c;
-                    if (x.grp == 0) a.lse[head] = L == 0.f ? -INFINITY : x.ref[g] * LN2 + logf(L);
+                    if (x.grp == 0) a.lse[head] = L == 0.f ? -INFINITY : log_sum(x.ref[g], L);
 #pragma unroll
                     for (int n = 0; n < NX; ++n)
 #pragma unroll
@@ -588,17 +591,121 @@ __global__ __launch_bounds__(64 * AT_WAVES) void kv_attend_kernel(const KvPool p
     if constexpr (MASS) flush(u1);
 }
 
-// Parts of one (sequence, head group): waves w0 .. w1, and where part w of them lies in the workspace.
-struct Parts {
-    int first, w0, w1;                   // first tile
-    __device__ __forceinline__ int slot(const Line& line, int w) const { return 2 * w + (line.begin(w) < first); }
-};
-
 // {reference exponent, sum} of two disjoint sets of weights as one.
 __device__ __forceinline__ float2 stat_join(float2 x, float2 y) {
     const float M = fmaxf(x.x, y.x), ref = M == -INFINITY ? 0.f : M;
     return float2{M, x.y * ex2(x.x - ref) + y.y * ex2(y.x - ref)};
 }
+
+// Short memories (an utterance's encoder outputs): a workgroup has a head group to itself, tile after tile dealt to its eight
+// waves, and everything that takes the long way a workspace and a second launch stays in its LDS: the waves' parts and the
+// scores of the whole memory, from which the weights are added to `mass`. Bound by its loads one after the other. Long way
+// against this one, with the weights, lengths from an eighth of the slots to all of them: 16 x 8 heads over 128 slots of 128,
+// bf16, four query heads each: 10.7 us, 6.5; 64 x 8: 15.8, 11.3; 64 x 8 over 512 slots of 64: 18.9, 13.7.
+constexpr int SHORT_WAVES = 8;
+
+// Tokens of memory that the short way takes: as many as have 64 KB of K, two rounds of the waves' tiles at D = 64, one at 128.
+// (Twice as many: 32 x 1 heads over 512 slots of 128, bf16: 10.6 us the long way, 11.2 the short; over 256 of fp32 10.7 and 12.5.)
+// And how many heads, to a CU: at D = 128 a CU holds one workgroup at a time (1024 heads, 4 a CU, over 256 slots, bf16: 25.7 us
+// the long way, 27.3 the short; 512: 16.5 and 15.0), at 64 three (4096 over 64 slots, no weights: 23.1 and 26.9; 2048: 14.9 and
+// 15.3, with weights 20.2 and 16.7). At D = 256 eight waves' registers do not fit a CU's (32 x 1 over 128 to 256 slots lost).
+constexpr int short_slots(int dtype, int dim) { return 65536 / (dim * (dtype == KV_F32 ? 4 : 2)); }
+constexpr int short_per_cu(int dim) { return dim == 64 ? 8 : dim == 128 ? 2 : 0; }
+
+template <int DT, int D, bool MASS>
+__global__ __launch_bounds__(64 * SHORT_WAVES) void kv_attend_short_kernel(const KvPool p, const KvTable tb, const KvAttend a) {
+    using Wave = AttendWave<DT, D, 1>;
+    constexpr int NW = SHORT_WAVES, HALF = NW / 2, TW = Wave::TW, VEC = Wave::VEC, NACC = Wave::NACC, STEP = NW * TW;
+    __shared__ f32x4 parts[HALF][NACC][64];          // a wave's accumulators, by lane
+    __shared__ float2 ml[NW][16];
+    __shared__ f32x4 score[MASS ? short_slots(DT, D) * 16 / 4 : 1];      // [tile][head][TW]
+    __shared__ float lse2[16];
+    Wave x(p, tb, a);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, nh = a.group;
+    const int len = clamp_len(a.lengths[b], tb.max_pages << p.page_shift, p.status, h == 0 && tid == 0);
+    const int64_t head0 = (int64_t)b * x.hq + h * a.group;
+    int t = wave * TW, kpage, vpage;
+    if (t < len) {
+        kpage = x.k_page(b, len, t);
+        vpage = x.v_page(b, len, t);
+        x.load_q(b, h);
+        x.load_k(h, t, kpage);
+        kpage = x.k_page(b, len, t + STEP);
+        for (;; t += STEP) {
+            const int kpage2 = x.k_page(b, len, t + 2 * STEP), vpage2 = x.v_page(b, len, t + STEP);
+            const bool last = t + STEP >= len;
+            x.load_v(h, t, vpage);
+            x.scores();
+            if (!last) x.load_k(h, t + STEP, kpage);
+            x.mask(len, t, vpage);
+            if (MASS && x.col < nh) x.put_scores(0, score + ((t / TW * 16 + x.col) * TW + Wave::NV * x.grp) / 4);
+            x.accumulate();
+            if (last) break;
+            kpage = kpage2;
+            vpage = vpage2;
+        }
+    }
+    // the waves' parts: the upper four into the lower four, those into the output
+    const float2 own = {x.exponent_of(0), x.sum_of(0)};
+    if (wave >= HALF) {
+        if (x.grp == 0) ml[wave][x.col] = own;
+#pragma unroll
+        for (int n = 0; n < NACC; ++n) parts[wave - HALF][n][x.lane] = x.acc[0][n];
+    }
+    __syncthreads();
+    if (wave < HALF) {
+        const float2 other = ml[wave + HALF][x.col], both = stat_join(own, other);
+        const float ref = both.x == -INFINITY ? 0.f : both.x, f = ex2(own.x - ref), g = ex2(other.x - ref);
+#pragma unroll
+        for (int n = 0; n < NACC; ++n) x.acc[0][n] = x.acc[0][n] * f + parts[wave][n][x.lane] * g;
+        if (x.grp == 0) ml[wave][x.col] = both;
+#pragma unroll
+        for (int n = 0; n < NACC; ++n) parts[wave][n][x.lane] = x.acc[0][n];
+    }
+    __syncthreads();
+    // {exponent, sum} of head c; a memory without tokens, or without a score above -inf, has sum 0
+    auto total = [&](int c) INLINE {
+        float2 y = ml[0][c];
+#pragma unroll
+        for (int i = 1; i < HALF; ++i) y = stat_join(y, ml[i][c]);
+        return y;
+    };
+    for (int i = tid; i < NACC * 64; i += 64 * NW) {
+        const int n = i >> 6, l = i & 63, c = l & 15;
+        if (c >= nh) continue;
+        const float2 y = total(c);
+        const float ref = y.x == -INFINITY ? 0.f : y.x, inv = y.y == 0.f ? 0.f : 1.f / y.y;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < HALF; ++w) o += parts[w][n][l] * ex2(ml[w][c].x - ref);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            store_out<DT>(a.out, (head0 + c) * D + n / VEC * 16 * VEC + (4 * (l >> 4) + e) * VEC + n % VEC, o[e] * inv);
+    }
+    if (tid < nh) {
+        const float2 y = total(tid);
+        const float ref = y.x == -INFINITY ? 0.f : y.x;
+        a.lse[head0 + tid] = y.y == 0.f ? -INFINITY : log_sum(ref, y.y);
+        lse2[tid] = y.y == 0.f ? 0.f : ref + __log2f(y.y);         // (no weight at all: every score is -inf)
+    }
+    if constexpr (MASS) {
+        __syncthreads();
+        float* mass = a.mass + ((int64_t)b * p.heads + h) * a.side_ld;
+        for (int s = tid; s < len; s += 64 * NW) {
+            const float* sc = (const float*)score + (s / TW * 16) * TW + s % TW;
+            float w = 0.f;
+            for (int c = 0; c < nh; ++c) w += ex2(sc[c * TW] - lse2[c]);
+            mass[s] += w;
+        }
+    }
+}
+
+// Parts of one (sequence, head group): waves w0 .. w1, and where part w of them lies in the workspace.
+struct Parts {
+    int first, w0, w1;                   // first tile
+    __device__ __forceinline__ int slot(const Line& line, int w) const { return 2 * w + (line.begin(w) < first); }
+};
 
 // The first `joins` workgroups join the parts of a (sequence, query head): one each, or, WAVES, one per wave. The rest
 // do mass_tokens tokens (a multiple of 1024) of mass[b][h] += sum over the query heads of h of exp(score - lse) each, from
@@ -701,7 +808,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         }
         o *= L == 0.f ? 0.f : 1.f / L;
         const int64_t head = (int64_t)b * hq + kvh * a.group + h0;
-        if (id == 0) a.lse[head] = L == 0.f ? -INFINITY : ref * LN2 + logf(L);
+        if (id == 0) a.lse[head] = L == 0.f ? -INFINITY : log_sum(ref, L);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int64_t at = head * D + 4 * d4 + e;
@@ -1223,8 +1330,14 @@ static int attend_groups(const KvPool& p, int B, int group, int max_pages) {
                                   attend_per_cu(p.dim) * kv_cus(p.device));
 }
 
+static bool attend_short(const KvPool& p, int B, int group, int max_pages) {
+    return group <= 16 && ((int64_t)max_pages << p.page_shift) <= short_slots(p.dtype, p.dim) &&
+           (int64_t)B * p.heads <= (int64_t)short_per_cu(p.dim) * kv_cus(p.device);
+}
+
 // {maximum, sum} and output of two parts per wave (the one it begins with, the one it ends with), and the scores
 size_t kv_attend_ws_bytes(const KvPool& p, int B, int group, int max_pages, bool mass) {
+    if (attend_short(p, B, group, max_pages)) return 0;
     const size_t parts = 2 * AT_WAVES * (size_t)attend_groups(p, B, group, max_pages), cols = (size_t)attend_columns(p, group), rows = std::min((size_t)group, cols);
     size_t n = parts * cols * sizeof(float2) + parts * rows * p.dim * sizeof(float);
     if (mass) n += (size_t)attend_tiles(p, B, group, max_pages) * rows * attend_tile(p.dtype) * sizeof(float);
@@ -1244,8 +1357,23 @@ static void attend_launch(const KvPool& p, const KvTable& tb, const KvAttend& a,
     else kv_attend_kernel<DT, D, false, 1><<<W, 64 * AT_WAVES, 0, s>>>(p, tb, a);
 }
 
+template <int DT, int D>
+static void attend_short_launch(const KvPool& p, const KvTable& tb, const KvAttend& a, hipStream_t s) {
+    const int grid = tb.B * p.heads, block = 64 * SHORT_WAVES;
+    if (a.mass) kv_attend_short_kernel<DT, D, true><<<grid, block, 0, s>>>(p, tb, a);
+    else kv_attend_short_kernel<DT, D, false><<<grid, block, 0, s>>>(p, tb, a);
+}
+
 template <int D>
 static void attend_both(const KvPool& p, const KvTable& tb, const KvAttend& a, int W, hipStream_t s) {
+    if constexpr (short_per_cu(D) > 0) {
+        if (attend_short(p, tb.B, a.group, tb.max_pages)) {
+            if (p.dtype == KV_F32) attend_short_launch<KV_F32, D>(p, tb, a, s);
+            else if (p.dtype == KV_BF16) attend_short_launch<KV_BF16, D>(p, tb, a, s);
+            else attend_short_launch<KV_F16, D>(p, tb, a, s);
+            return;
+        }
+    }
     if (p.dtype == KV_F32) attend_launch<KV_F32, D>(p, tb, a, W, s);
     else if (p.dtype == KV_BF16) attend_launch<KV_BF16, D>(p, tb, a, W, s);
     else attend_launch<KV_F16, D>(p, tb, a, W, s);

@@ -43,6 +43,7 @@ class KvCache:
         self.device, self.dtype = k_pages.device, k_pages.dtype
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._none = torch.empty(16, dtype=torch.uint8, device=self.device)
         p = _lib.TacoKvPool()
         p.struct_size = ctypes.sizeof(p)
         p.device, p.dtype = self.device.index, _DTYPES[self.dtype]
@@ -123,6 +124,8 @@ class KvCache:
             if len(self._need) >= 256:
                 self._need.clear()
             self._need[(query, sizes)] = need
+        if need <= 16:                               # the least there is: the call uses none
+            return self._none, need
         return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
     def _stream(self):

@@ -85,6 +85,24 @@ def test_attend_ragged(dtype, d, hkv, group):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('d', [64, 128, 256])
+@pytest.mark.parametrize('hkv,group', [(1, 1), (5, 1), (2, 2), (3, 7), (1, 16), (1, 17)])
+@pytest.mark.parametrize('slots', [64, 160, 256, 512])
+def test_attend_short_memories(dtype, d, hkv, group, slots):
+    """Tables of few slots, whose rows one workgroup can hold: every length about the sizes it deals out."""
+    lens = sorted({n for k in (0, 8, 16, 32, 64, 96, 100, 128, 150, 256, 500, 512) for n in (k - 1, k, k + 1) if 0 <= n <= slots})
+    cache, table, lengths = _make(d + slots, lens, hkv, d, 32 if slots % 32 == 0 and d > 64 else 8, dtype, slots=slots)
+    _check_attend(cache, table, lengths, _q(group, len(lens), hkv * group, d, dtype, size=2.0), with_mass=slots != 160, mass0=1.5 if slots == 64 else 0.0)
+
+
+@pytest.mark.parametrize('d,batch', [(64, 250), (64, 270), (128, 60), (128, 70)])
+def test_attend_many_short_memories(d, batch):
+    lens = [(7 * b) % 41 for b in range(batch)]
+    cache, table, lengths = _make(d + batch, lens, 8, d, 8, 'bfloat16')
+    _check_attend(cache, table, lengths, _q(batch, batch, 16, d, 'bfloat16'))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('page', [8, 16, 32, 64, 128, 256])
 def test_attend_page_sizes(dtype, page):
     lens = [page, page - 1, page + 1, 3 * page + 5, 1, 2 * page]
@@ -147,12 +165,13 @@ def test_attend_many_small_weights_next_to_a_large_one(dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-def test_attend_infinite_scores(dtype):
+@pytest.mark.parametrize('group,slots', [(3, 150), (1, 150), (3, 3000), (1, 3000)])
+def test_attend_infinite_scores(dtype, group, slots):
     """Tokens whose score is -inf weigh nothing; a row of them is a row without tokens."""
     import torch
     lens = [150, 150, 40]
-    cache, table, lengths = _make(15, lens, 1, 64, 16, dtype)
-    q = _q(16, 3, 3, 64, dtype)
+    cache, table, lengths = _make(15, lens, 1, 64, 16, dtype, slots=slots)
+    q = _q(16, 3, group, 64, dtype)
     q[..., 0] = 1.0
     for b in (0, 2):
         for t in range(lens[b]):
@@ -172,28 +191,30 @@ def test_attend_infinite_scores(dtype):
     cache.status()
 
 
-def test_attend_nan_stays_in_its_row():
+@pytest.mark.parametrize('group,slots', [(2, 200), (1, 200), (2, 3000)])
+def test_attend_nan_stays_in_its_row(group, slots):
     import torch
     lens = [200, 200]
-    cache, table, lengths = _make(17, lens, 2, 64, 16, 'bfloat16')
-    q = _q(18, 2, 4, 64, 'bfloat16')
+    cache, table, lengths = _make(17, lens, 2, 64, 16, 'bfloat16', slots=slots)
+    q = _q(18, 2, 2 * group, 64, 'bfloat16')
     clean, _ = cache.attend(q, table, lengths)
     cache.v_pages[int(table[1, 4]), 1, 3, 5] = math.nan
     out, lse = cache.attend(q, table, lengths)
     hit = torch.zeros_like(out, dtype=torch.bool)
-    hit[1, 2:, 5] = True
+    hit[1, group:, 5] = True
     assert torch.equal(torch.isnan(out), hit) and torch.equal(out[~hit], clean[~hit])
     cache.k_pages[int(table[0, 2]), 0, 1, 7] = math.nan
     out, lse = cache.attend(q, table, lengths)
-    assert torch.isnan(out[0, :2]).all() and torch.isnan(lse[0, :2]).all() and not torch.isnan(out[0, 2:]).any()
+    assert torch.isnan(out[0, :group]).all() and torch.isnan(lse[0, :group]).all() and not torch.isnan(out[0, group:]).any()
 
 
-def test_attend_bad_pages_and_lengths_are_masked():
+@pytest.mark.parametrize('group,slots', [(2, 100), (1, 100), (2, 3000)])
+def test_attend_bad_pages_and_lengths_are_masked(group, slots):
     import torch
     from tacotron_amd.engine import TacoError
     lens = [100, 40, 64, 33]
-    cache, table, lengths = _make(19, lens, 2, 64, 16, 'float32')
-    q = _q(20, 4, 4, 64, 'float32')
+    cache, table, lengths = _make(19, lens, 2, 64, 16, 'float32', slots=slots)
+    q = _q(20, 4, 2 * group, 64, 'float32')
     good, good_lse = cache.attend(q, table, lengths)
     bad = table.clone()
     bad[0, 2], bad[0, 5] = cache.num_pages, -7
@@ -205,8 +226,9 @@ def test_attend_bad_pages_and_lengths_are_masked():
     rows = [t for t in range(100) if t // 16 not in (2, 5)]
     for h in range(2):
         k, v = (torch.from_numpy(R.rows_of(x, table, 0, h, 100)[rows]) for x in (cache.k_pages, cache.v_pages))
-        p = torch.softmax(q[0, 2 * h:2 * h + 2].double().cpu() @ k.t() / 8, 1)
-        assert (out[0, 2 * h:2 * h + 2].double().cpu() - p @ v).abs().max() < 1e-5
+        mine = slice(group * h, group * h + group)
+        p = torch.softmax(q[0, mine].double().cpu() @ k.t() / 8, 1)
+        assert (out[0, mine].double().cpu() - p @ v).abs().max() < 1e-5
         assert (mass[0, h, rows].double().cpu() - p.sum(0)).abs().max() < 1e-5
     assert (mass[0, :, 32:48] == 0).all() and torch.equal(out[1:], good[1:]) and torch.equal(lse[1:], good_lse[1:])
     # every page of a row bad: a row without tokens
