@@ -336,8 +336,8 @@ int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int64_t table_l
                    taco_stream_t stream);
 
 /* Every (sequence, kv head) is cut to n = min(lengths[b], budget) tokens: the `recent` newest by position (those above
- * the greatest position - recent), then the greatest masses; of equal masses the lower slot stays, NaN counts as the
- * greatest. Kept slots below n stay where they are; the empty slots below n take the kept ones from n on, both in
+ * the greatest position - recent; the lower slots, should positions repeat and more than n be such), then the greatest
+ * masses; of equal masses the lower slot stays, NaN counts as the greatest. Kept slots below n stay where they are; the empty slots below n take the kept ones from n on, both in
  * ascending order, so no more rows move than have to (one per head when a sequence is one over its budget) and attention,
  * which does not depend on the order of slots, goes on. positions says which token a slot holds.
  *   mass, positions [B, kv_heads, side_ld] -> mass_out, positions_out: slots >= n get 0 and -1

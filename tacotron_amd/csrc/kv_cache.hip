@@ -1156,6 +1156,75 @@ __device__ __forceinline__ void move_rows(const KvPool& p, const KvTable& tb, co
     }
 }
 
+// Greatest of a waves' value in wave_x, one of each, over the workgroup.
+__device__ __forceinline__ int waves_max(const int* wave_x, int none) {
+    const int lane = threadIdx.x & 63;
+    return wave_max(lane < EV_WAVES ? wave_x[lane] : none);
+}
+
+// A head one token over its budget, as every step of a decoder that holds one leaves it: the token that goes is the least key's,
+// of equal ones the last, found in two barriers without a select, and at most one row moves, that of slot n, which is loaded
+// meanwhile. (32 x 8 heads of 2049 tokens: 11.0 us by the select, 6.5 here.)
+template <int R>
+__device__ __forceinline__ void drop_one(SelectShared& sh, const KvPool& p, const KvTable& tb, Head& a, int recent, int h, int b) {
+    constexpr int NONE = -0x7fffffff - 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
+    const int per = (a.len + EV_THREADS - 1) / EV_THREADS, vecs = (p.dim * p.esize) >> 4, mask = p.page_size - 1;
+    const int32_t* table = tb.table + (int64_t)b * tb.ld;
+    Slots<R> x;
+    x.load(a, wave * per * 64 + lane, min(a.len, (wave + 1) * per * 64), per);
+    const bool is_k = tid < vecs, mover = tid < 2 * vecs;      // a piece of row n each
+    const int pf = table[n >> p.page_shift], c = is_k ? tid : tid - vecs;
+    const bool bad_from = (unsigned)pf >= (unsigned)p.num_pages;
+    char* pool = (char*)(is_k ? p.k : p.v);
+    auto at = [&](int page, int s) INLINE {
+        const int64_t k = slot_off(p.k_st, page, h, s & mask), v = slot_off(p.v_st, page, h, s & mask);
+        return reinterpret_cast<u32x4*>(pool + (is_k ? k : v) * p.esize) + c;
+    };
+    u32x4 piece = {};
+    if (mover && !bad_from) piece = *at(pf, n);
+    if (recent > 0) {
+        const int newest = wave_max(x.newest(per));
+        if (lane == 0) sh.wave_a[wave] = newest;
+        __syncthreads();
+        a.protect(waves_max(sh.wave_a, NONE), recent);
+    }
+    int least = NONE, slot = -1;                     // the key's bits in descending order, as a number with a sign
+    for_rows<R>(per, [&](auto i) INLINE {
+        const uint32_t k = x.key(a, i, per);
+        const int v = (int)(~k ^ 0x80000000u);
+        if (k != 0u && v >= least) { least = v; slot = x.slot(i); }
+    });
+    int m = wave_max(least);
+    slot = wave_max(least == m ? slot : -1);
+    if (lane == 0) { sh.hist[wave] = (uint32_t)m; sh.wave_b[wave] = slot; }
+    __syncthreads();
+    least = lane < EV_WAVES ? (int)sh.hist[lane] : NONE;
+    m = wave_max(least);
+    const int gone = wave_max(lane < EV_WAVES && least == m ? sh.wave_b[lane] : -1);
+    const bool copy = a.mass_out != a.mass, copy_pos = a.pos_out != a.pos;
+    for_rows<R>(per, [&](auto i) INLINE {
+        const int s = x.slot(i);
+        if (i >= per || s >= x.stop) return;
+        if (s == n) {
+            if (gone != n) { a.mass_out[gone] = x.mass[i]; a.pos_out[gone] = x.pos[i]; }
+            a.mass_out[n] = 0.f;
+            a.pos_out[n] = -1;
+        } else if (s != gone) {
+            if (copy) a.mass_out[s] = x.mass[i];
+            if (copy_pos) a.pos_out[s] = x.pos[i];
+        }
+    });
+    if (tid == 0) a.counts[0] = n;                   // nothing is left to move
+    if (!mover || gone == n) return;
+    const int pt = table[gone >> p.page_shift];
+    if (bad_from || (unsigned)pt >= (unsigned)p.num_pages) {
+        if (tid == 0) atomicOr(p.status, KV_BAD_PAGE);
+        return;
+    }
+    *at(pt, gone) = piece;
+}
+
 // One workgroup per (sequence, kv head). The n-th greatest key by a radix select of 11 + 11 + 10 bits, then one pass in
 // slot order. Masses and positions stay in registers, so they are read once, together; what is left are LDS counters and a
 // dozen barriers, which bound it: 10 us at 2049 tokens, 15 at 8192, a head to a CU.
@@ -1163,15 +1232,19 @@ template <bool MOVE>
 __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, const KvTable tb, const KvEvict a) {
     __shared__ SelectShared sh;
     Head head(p, tb, a, blockIdx.x, blockIdx.y, blockIdx.x == 0 && threadIdx.x == 0);
-    if (head.len > head.n) {
+    const bool one = head.len == head.n + 1;
+    if (one) {
+        if (head.len <= 4 * EV_THREADS) drop_one<4>(sh, p, tb, head, a.recent, blockIdx.x, blockIdx.y);
+        else drop_one<EV_ROWS>(sh, p, tb, head, a.recent, blockIdx.x, blockIdx.y);
+    } else if (head.len > head.n) {
         if (head.len <= 4 * EV_THREADS) select_head<4>(sh, head, a.recent);
         else select_head<EV_ROWS>(sh, head, a.recent);
     }
     keep_all(head, 0, a.side_ld);
     if constexpr (MOVE) {
-        __syncthreads();                             // the lists and counts of this workgroup
+        if (!one) __syncthreads();                   // the lists and counts of this workgroup
         if (blockIdx.x == 0 && threadIdx.x == 0) a.lengths_out[blockIdx.y] = head.n;
-        move_rows(p, tb, a, blockIdx.x, blockIdx.y, head.counts[0], head.n, threadIdx.x, EV_THREADS);
+        if (!one) move_rows(p, tb, a, blockIdx.x, blockIdx.y, head.counts[0], head.n, threadIdx.x, EV_THREADS);
     }
 }
 

@@ -55,14 +55,14 @@ def attend(q, k_pages, v_pages, table, lengths, scale):
 
 
 def survivors(mass, pos, n, recent):
-    """Slots of one head that are kept, ascending: the newest `recent` positions, then the greatest masses (NaN greatest,
-    equal ones by slot)."""
+    """Slots of one head that are kept, ascending: the newest `recent` positions (by slot, should positions repeat and more
+    than n be among them), then the greatest masses (NaN greatest, equal ones by slot)."""
     L = len(mass)
     if n == L:
         return np.arange(L)
     new = pos.astype(np.int64) > int(pos.max()) - recent
-    m = np.where(np.isnan(mass), np.inf, mass.astype(np.float64))
-    return np.sort(np.lexsort((np.arange(L), -m, ~np.isnan(mass), ~new))[:n])
+    m = np.where(np.isnan(mass) | new, np.inf, mass.astype(np.float64))
+    return np.sort(np.lexsort((np.arange(L), -m, ~(np.isnan(mass) | new), ~new))[:n])
 
 
 def evict(k, v, mass, pos, lengths, budget, recent):

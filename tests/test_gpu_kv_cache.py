@@ -460,6 +460,68 @@ def test_evict(inplace, dtype, d, hkv, page, budget, recent, masses):
 
 
 @pytest.mark.parametrize('inplace', [False, True])
+@pytest.mark.parametrize('masses', ['random', 'ties', 'odd', 'equal', 'last'])
+@pytest.mark.parametrize('dtype,d,hkv,page,budget,recent', [
+    ('float32', 64, 1, 8, 1, 0), ('float32', 64, 1, 8, 1, 1), ('float32', 256, 2, 16, 63, 5), ('bfloat16', 128, 3, 16, 64, 64),
+    ('float16', 64, 2, 8, 1023, 0), ('bfloat16', 256, 1, 32, 1024, 100), ('bfloat16', 64, 2, 16, 4095, 4095),
+    ('float32', 64, 1, 16, 4096, 1), ('float16', 128, 1, 256, 16383, 300)])
+def test_evict_one_over(inplace, masses, dtype, d, hkv, page, budget, recent):
+    """Rows one token over the budget beside others; a table that ends with the token, and one that does not."""
+    import torch
+    for lens in ([budget + 1], [budget + 1, budget, 0, budget + 1], [budget + 1, min(2 * budget + 3, 16384), budget + 1]):
+        cache, table, lengths = _make(budget, lens, hkv, d, page, dtype)
+        slots = table.shape[1] * page
+        g = torch.Generator().manual_seed(budget + len(lens))
+        mass = torch.rand(len(lens), hkv, slots, generator=g) ** 3
+        pos = torch.stack([torch.stack([torch.randperm(slots, generator=g) for _ in range(hkv)]) for _ in lens]).to(torch.int32)
+        if masses == 'ties':
+            mass = torch.floor(mass * 3)
+        if masses == 'equal':
+            mass[:] = 0.25
+        if masses == 'last':                 # the token that goes is the one in the last slot
+            mass[:, :, budget] = 0.0
+            pos[:, :, budget] = -1
+        if masses == 'odd':
+            pick = torch.rand(mass.shape, generator=g)
+            mass[pick < 0.3] = float('nan')
+            mass[(pick > 0.3) & (pick < 0.6)] = float('inf')
+            mass[(pick > 0.6) & (pick < 0.65)] = -float('inf')
+            mass[pick > 0.9] = -0.0
+            pos //= 2
+        _check_evict(cache, table, lengths, mass.cuda(), pos.cuda(), budget, recent, inplace)
+
+
+@pytest.mark.parametrize('gone', [70, 150, 200])
+def test_evict_one_over_bad_page(gone):
+    """A bad page under the row that moves, or under the gap: nothing is written there, side tables stay consistent."""
+    import torch
+    from tacotron_amd.engine import TacoError
+    for hurt in (70, 200):
+        cache, table, lengths = _make(51, [201], 2, 64, 16, 'bfloat16')
+        mass = torch.ones(1, 2, 208, device='cuda')
+        mass[0, :, gone] = 0.0
+        pos = torch.arange(208, dtype=torch.int32, device='cuda').expand(1, 2, 208).contiguous()
+        bad = table.clone()
+        bad[0, hurt // 16] = cache.num_pages
+        before, rows = cache.k_pages.clone(), _flat(cache, cache.v_pages, table, 0, 1, 201).clone()
+        n, m, p = cache.evict(bad, lengths, mass, pos, 200, 0)
+        if gone != 200 and hurt in (gone, 200):
+            with pytest.raises(TacoError, match='page id'):
+                cache.status()
+            assert torch.equal(torch.nan_to_num(before.float(), 5.0), torch.nan_to_num(cache.k_pages.float(), 5.0))
+        else:
+            cache.status()
+            if gone != 200:
+                rows[gone] = rows[200]
+            assert torch.equal(_flat(cache, cache.v_pages, table, 0, 1, 200), rows[:200])
+        want = list(range(200))
+        if gone != 200:
+            want[gone] = 200
+        assert n.tolist() == [200] and p[0, 1, :200].tolist() == want
+        assert (p[..., 200:] == -1).all() and (m[..., 200:] == 0).all() and (m[..., :200] == 1).all()
+
+
+@pytest.mark.parametrize('inplace', [False, True])
 def test_evict_long(inplace):
     import torch
     lens = [70003, 8193]
