@@ -922,6 +922,7 @@ template <int R>
 struct Slots {
     float mass[R];
     int pos[R];
+    uint32_t key[R];                                 // 0 for no slot
     int first, stop;                                 // slots from stop on are none
     // (rows behind per, and slots behind stop, read the last slot; the wave has slots, or nothing is read)
     __device__ __forceinline__ void load(const Head& h, int first_, int stop_, int per) {
@@ -942,12 +943,19 @@ struct Slots {
         });
         return x;
     }
-    // 0 for no slot
-    __device__ __forceinline__ uint32_t key(const Head& h, int i, int per) const {
-        const uint32_t k = pos[i] > h.border ? 0xffffffffu : mass_key(mass[i]);
-        return i < per && slot(i) < stop ? k : 0u;
+    // Made once, each of the passes below would be bound by making them again.
+    __device__ __forceinline__ void make_keys(const Head& h, int per) {
+        for_rows<R>(per, [&](auto i) INLINE {
+            const uint32_t k = pos[i] > h.border ? 0xffffffffu : mass_key(mass[i]);
+            key[i] = i < per && slot(i) < stop ? k : 0u;
+        });
     }
 };
+
+// n and the set bits of a wave's mask below this lane's.
+__device__ __forceinline__ int lanes_below(unsigned long long mask, int n) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, (uint32_t)n));
+}
 
 // Counts a key's digit if `in`. Equal digits side by side (fresh tokens, protected ones) would queue for one counter: where
 // a wave has only one digit it adds once.
@@ -1034,7 +1042,7 @@ __device__ __forceinline__ void emit(SelectShared& sh, const Head& a, const Slot
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int g = 0, e0 = 0;
     for_rows<R>(per, [&](auto i) INLINE {
-        const uint32_t k = x.key(a, i, per);
+        const uint32_t k = x.key[i];
         g += __popcll(__ballot(k > thr));
         e0 += __popcll(__ballot(k == thr));
     });
@@ -1044,13 +1052,12 @@ __device__ __forceinline__ void emit(SelectShared& sh, const Head& a, const Slot
         gt += w < wave ? sh.wave_a[w] : 0;
         eq += w < wave ? sh.wave_b[w] : 0;
     }
-    const unsigned long long low = (1ull << lane) - 1;
     const bool copy = a.mass_out != a.mass, copy_pos = a.pos_out != a.pos;
     for_rows<R>(per, [&](auto i) INLINE {
         const int s = x.slot(i);
-        const uint32_t k = x.key(a, i, per);
+        const uint32_t k = x.key[i];
         const unsigned long long bg = __ballot(k > thr), be = __ballot(k == thr);
-        const int e = eq + __popcll(be & low), before = gt + __popcll(bg & low) + min(e, need);
+        const int e = lanes_below(be, eq), before = lanes_below(bg, gt) + min(e, need);
         const bool keep = k > thr || (k == thr && e < need);
         gt += __popcll(bg);
         eq += __popcll(be);
@@ -1087,14 +1094,14 @@ template <int R>
 __device__ __forceinline__ void list_keys(const Head& a, const Slots<R>& x, int per, uint32_t digit, uint32_t* list, int* n) {
     const int lane = threadIdx.x & 63;
     for_rows<R>(per, [&](auto i) INLINE {
-        const uint32_t k = x.key(a, i, per);
+        const uint32_t k = x.key[i];
         const bool in = k != 0u && k >> 21 == digit;
         const unsigned long long who = __ballot(in);
         if (who) {
             int at = 0;
             if (lane == 0) at = atomicAdd(n, __popcll(who));
             at = __builtin_amdgcn_readfirstlane(at);
-            if (in) list[at + __popcll(who & ((1ull << lane) - 1))] = k;
+            if (in) list[lanes_below(who, at)] = k;
         }
     });
 }
@@ -1110,7 +1117,8 @@ __device__ __forceinline__ void select_head(SelectShared& sh, Head& a, int recen
     clear_hist(sh);
     __syncthreads();
     if (recent > 0) a.protect(block_max(sh, x.newest(per)), recent);
-    for_rows<R>(per, [&](auto i) INLINE { const uint32_t k = x.key(a, i, per); count_digit(sh, k != 0u, k >> 21); });
+    x.make_keys(a, per);
+    for_rows<R>(per, [&](auto i) INLINE { count_digit(sh, x.key[i] != 0u, x.key[i] >> 21); });
     __syncthreads();
     pick_digit(sh, a.n);
     uint32_t thr = sh.digit << 21;
@@ -1121,7 +1129,7 @@ __device__ __forceinline__ void select_head(SelectShared& sh, Head& a, int recen
     __syncthreads();
     if (few)
         pick_rest(sh, [&](auto f) INLINE { for (int i = tid; i - lane < sh.listed; i += EV_THREADS) f(i < sh.listed ? sh.list[i] : 0u); }, &thr, &need);
-    else pick_rest(sh, [&](auto f) INLINE { for_rows<R>(per, [&](auto i) INLINE { f(x.key(a, i, per)); }); }, &thr, &need);
+    else pick_rest(sh, [&](auto f) INLINE { for_rows<R>(per, [&](auto i) INLINE { f(x.key[i]); }); }, &thr, &need);
     emit<R>(sh, a, x, per, thr, need, 0, 0);
 }
 
@@ -1189,9 +1197,10 @@ __device__ __forceinline__ void drop_one(SelectShared& sh, const KvPool& p, cons
         __syncthreads();
         a.protect(waves_max(sh.wave_a, NONE), recent);
     }
+    x.make_keys(a, per);
     int least = NONE, slot = -1;                     // the key's bits in descending order, as a number with a sign
     for_rows<R>(per, [&](auto i) INLINE {
-        const uint32_t k = x.key(a, i, per);
+        const uint32_t k = x.key[i];
         const int v = (int)(~k ^ 0x80000000u);
         if (k != 0u && v >= least) { least = v; slot = x.slot(i); }
     });
@@ -1292,8 +1301,9 @@ __global__ __launch_bounds__(EV_THREADS) void kv_select_chunk_kernel(const KvPoo
             for (int i = lane; i < chunks; i += 64) newest = max(newest, ws.newest[i]);
         head.protect(block_max(sh, newest), a.recent);
     }
+    x.make_keys(head, R);
     if (STAGE == 1) {
-        for_rows<R>(R, [&](auto i) INLINE { const uint32_t k = x.key(head, i, R); count_digit(sh, k != 0u, k >> 21); });
+        for_rows<R>(R, [&](auto i) INLINE { count_digit(sh, x.key[i] != 0u, x.key[i] >> 21); });
         __syncthreads();
         for (int i = tid; i < 2048; i += EV_THREADS) ws.hist[(int64_t)c * 2048 + i] = sh.hist[i];
         return;
