@@ -1139,9 +1139,9 @@ __device__ __forceinline__ void move_rows(const KvPool& p, const KvTable& tb, co
     const int32_t* gaps = a.lists + row * 2 * a.list_ld;
     const int32_t* late = gaps + a.list_ld + low;
     const int32_t* table = tb.table + (int64_t)b * tb.ld;
-    const int vecs = (p.dim * p.esize) >> 4, mask = p.page_size - 1;
+    const int vecs = (p.dim * p.esize) >> 4, vec_shift = 31 - __builtin_clz(vecs), mask = p.page_size - 1;
     for (int64_t i = first; i < (int64_t)(n - low) * vecs; i += step) {
-        const int c = (int)(i % vecs), r = (int)(i / vecs);
+        const int c = (int)i & (vecs - 1), r = (int)(i >> vec_shift);
         const int to = gaps[r], from = late[r];
         if (c == 0) {
             const int64_t o = row * a.side_ld;
