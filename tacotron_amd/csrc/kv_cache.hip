@@ -739,12 +739,14 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         kvh = i / chunks % p.heads;
         t0 = i % chunks * mass_tokens;
     }
-    const int len = max(0, min(a.lengths[b], cap));
+    b = __builtin_amdgcn_readfirstlane(b);
+    const int len64 = lane < tb.B ? max(0, min(a.lengths[lane], cap)) : 0;
+    const int len = b < 64 ? __builtin_amdgcn_readlane(len64, b) : max(0, min(a.lengths[b], cap));
     if (t0 >= len) return;
     const int nb = (len + tw - 1) / tw;
     if (join && nb == 1) return;                     // a single tile is never in parts
-    int total = 0, before = 0;
-    for (int i = lane; i < tb.B; i += 64) {
+    int total = (len64 + tw - 1) / tw, before = lane < b ? total : 0;
+    for (int i = lane + 64; i < tb.B; i += 64) {
         const int n = tiles_of(tb, a.lengths, i, cap, tw);
         total += n;
         before += i < b ? n : 0;
@@ -770,6 +772,18 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
         const Parts q = parts_of(h0 / cols);
         if (q.w0 == q.w1) return;
         const int c = h0 % cols, n = q.w1 - q.w0 + 1;
+        const int id = WAVES ? lane : tid, d4 = id % COLS, k = id / COLS;
+        f32x4 v[AHEAD];
+        float f[AHEAD];
+        auto load = [&](int i) INLINE {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int slot = q.slot(line, q.w0 + min(i + j * ROWS, n - 1));      // (beyond the last part: not added)
+                v[j] = *reinterpret_cast<const f32x4*>(a.part_out + ((int64_t)slot * a.score_rows + c) * D + 4 * d4);
+                f[j] = a.part_ml[slot * cols + c].x;
+            }
+        };
+        load(k);                                     // beside the statistics
         float2 x = stats(q, c, WAVES ? lane : tid, WAVES ? 64 : 256);
         if (!WAVES) {
             if (lane == 0) wave_stat[wave] = x;
@@ -777,20 +791,14 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTa
             x = stat_join(stat_join(wave_stat[0], wave_stat[1]), stat_join(wave_stat[2], wave_stat[3]));
         }
         const float ref = x.x == -INFINITY ? 0.f : x.x, L = x.y;
-        const int id = WAVES ? lane : tid, d4 = id % COLS, k = id / COLS;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int i = k; i < n; i += AHEAD * ROWS) {
-            f32x4 v[AHEAD];
-            float f[AHEAD];
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                const int slot = q.slot(line, q.w0 + min(i + j * ROWS, n - 1));      // (beyond the last part: not added)
-                v[j] = *reinterpret_cast<const f32x4*>(a.part_out + ((int64_t)slot * a.score_rows + c) * D + 4 * d4);
-                f[j] = a.part_ml[slot * cols + c].x;
-            }
+        for (int i = k;;) {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
                 if (i + j * ROWS < n) o += v[j] * ex2(f[j] - ref);
+            i += AHEAD * ROWS;
+            if (i >= n) break;
+            load(i);
         }
         if constexpr (WAVES) {
 #pragma unroll
