@@ -712,7 +712,7 @@ struct Parts {
 // the scores that kv_attend_kernel left. The lse of a head in parts is computed by whoever needs it (a few values), so
 // that both fit one launch. Short work that waits for one dependent load after the other, so every step loads all it needs
 // at once: a part's {exponent, sum} per lane, eight or sixteen rows of the parts' outputs per lane, four tokens of a head's
-// scores per lane. (5 us where there is little to do; 36 us for the 126 MB of scores and masses of 32 sequences up to 32768.)
+// scores per lane, the first of them beside the statistics. (5 us where there is little to do; 31 us for the 126 MB of scores and masses of 32 sequences up to 32768.)
 template <int D, bool WAVES>
 __global__ __launch_bounds__(256) void kv_join_kernel(const KvPool p, const KvTable tb, const KvAttend a, int W, int tw, int joins,
                                                       int mass_tokens) {
@@ -1180,7 +1180,7 @@ __device__ __forceinline__ int waves_max(const int* wave_x, int none) {
 
 // A head one token over its budget, as every step of a decoder that holds one leaves it: the token that goes is the least key's,
 // of equal ones the last, found in two barriers without a select, and at most one row moves, that of slot n, which is loaded
-// meanwhile. (32 x 8 heads of 2049 tokens: 11.0 us by the select, 6.5 here.)
+// meanwhile. (32 x 8 heads of 2049 tokens: 11.3 us by the select, 6.3 here.)
 template <int R>
 __device__ __forceinline__ void drop_one(SelectShared& sh, const KvPool& p, const KvTable& tb, Head& a, int recent, int h, int b) {
     constexpr int NONE = -0x7fffffff - 1;
@@ -1244,7 +1244,7 @@ __device__ __forceinline__ void drop_one(SelectShared& sh, const KvPool& p, cons
 
 // One workgroup per (sequence, kv head). The n-th greatest key by a radix select of 11 + 11 + 10 bits, then one pass in
 // slot order. Masses and positions stay in registers, so they are read once, together; what is left are LDS counters and a
-// dozen barriers, which bound it: 10 us at 2049 tokens, 15 at 8192, a head to a CU.
+// dozen barriers, which bound it: a head to a CU, 14 us at 8192 tokens, 4 of them the loads, 4 the last pass.
 template <bool MOVE>
 __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, const KvTable tb, const KvEvict a) {
     __shared__ SelectShared sh;
@@ -1269,7 +1269,7 @@ __global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const KvPool p, c
 // the head's threshold for itself from what the one before left: the chunks' newest positions, the chunks' histograms of the
 // first digit, the chunks' lists of the keys that share the threshold's first digit. Sums over chunks before
 // its own give it the ranks of its slots, so nothing waits for anything and no counter is shared. (32 heads of 65536 tokens:
-// 5 + 5 + 9 + 19 us.)
+// 5 + 5 + 8 + 17 us.)
 struct ChunkWork {
     int32_t* newest;                     // [chunks]
     uint32_t* hist;                      // [chunks][2048]
@@ -1498,8 +1498,8 @@ static size_t kv_evict_list(const KvPool& p, int max_pages, int budget) {
     return (size_t)std::min<int64_t>(budget, (int64_t)max_pages << p.page_shift);
 }
 
-// Chunks of the long select, 0 where a workgroup holds a head. (One launch against four: an eviction of 32 heads takes 25
-// us and 37 at 8192 slots, 32 and 37 at 16384; at 65536 a workgroup a head took 168, the chunks take 65.)
+// Chunks of the long select, 0 where a workgroup holds a head. (One launch against four: an eviction of 32 heads to half
+// its tokens takes 23 us and 36 at 8192 slots, 37 and 45 at 16384; at 65536 a workgroup a head took 168 and the chunks 65.)
 static int64_t kv_evict_chunks(const KvPool& p, int max_pages) {
     const int64_t cap = (int64_t)max_pages << p.page_shift;
     return cap <= EV_ROWS * EV_THREADS ? 0 : (cap + EV_CHUNK - 1) / EV_CHUNK;
