@@ -40,7 +40,7 @@ class KvCache:
             raise TacoError('KvCache needs a GPU; there is no CPU path')
         self.lib = _lib.load_library()
         self.k_pages, self.v_pages = k_pages, v_pages
-        self.device, self.dtype = k_pages.device, k_pages.dtype
+        self.device, self.dtype, self._index = k_pages.device, k_pages.dtype, k_pages.device.index
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
         own = torch.zeros(8, dtype=torch.int32, device=self.device)
         self._status, self._none = own[:1], own[4:]  # _none: 16 bytes, the workspace of calls that use none
@@ -81,20 +81,26 @@ class KvCache:
         if rc != 0:
             raise TacoError(_lib.last_error())
 
+    # (get_device, an int, is -1 for host tensors; comparing devices builds objects)
     def _ints(self, t, name, B):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or t.shape[0] != B:
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != self._index or t.shape != (B,):
             raise TacoError('%s must be an int32 tensor [%d] on %s' % (name, B, self.device))
         return t if t.is_contiguous() else t.contiguous()
 
     def _table(self, t, B=None):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device or t.dim() != 2 or not t.numel():
+        """The page table, rows contiguous, its rows' distance and its shape."""
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != self._index or t.dim() != 2 or not t.numel():
             raise TacoError('page_table must be an int32 tensor [B, max_pages] on %s' % self.device)
-        if B is not None and t.shape[0] != B:
+        n, max_pages = t.shape
+        if B is not None and n != B:
             raise TacoError('page_table must have a row for each of the %d sequences' % B)
-        return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+        ld, one = t.stride()
+        if one != 1 or ld < max_pages:
+            t, ld = t.contiguous(), max_pages
+        return t, ld, n, max_pages
 
     def _side(self, t, name, dtype, B, slots):
-        if isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == self.device and t.dim() == 3 and t.is_contiguous():
+        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self._index and t.dim() == 3 and t.is_contiguous():
             n, h, ld = t.shape
             if n == B and h == self.kv_heads and ld >= slots:
                 return ld
@@ -103,7 +109,7 @@ class KvCache:
 
     def _rows(self, t, name):
         """Rows of head_dim elements: contiguous, 16-byte aligned, or copied to be. Returns it and its strides."""
-        if t.dtype != self.dtype or t.device != self.device:
+        if t.dtype is not self.dtype or t.get_device() != self._index:
             raise TacoError('%s must be %s on %s, as the pool' % (name, str(self.dtype)[6:], self.device))
         st = t.stride()
         bits = t.data_ptr()
@@ -130,7 +136,7 @@ class KvCache:
 
     def _stream(self):
         # the handle alone: torch.cuda.current_stream builds an object around it
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        return torch._C._cuda_getCurrentRawStream(self._index)
 
     # ---- the operators
     def append(self, k, v, page_table, starts, counts=None, first=None, mass=None, positions=None):
@@ -143,8 +149,8 @@ class KvCache:
         if k.shape != v.shape:
             raise TacoError('k and v must have the same shape')
         B, T = k.shape[:2]
-        (k, ks), (v, vs), table = self._rows(k, 'k'), self._rows(v, 'v'), self._table(page_table, B)
-        max_pages = table.shape[1]
+        (k, ks), (v, vs) = self._rows(k, 'k'), self._rows(v, 'v')
+        table, table_ld, _, max_pages = self._table(page_table, B)
         ld = slots = max_pages * self.page_size
         starts = self._ints(starts, 'starts', B)
         counts = self._ints(counts, 'counts', B) if counts is not None else None
@@ -158,7 +164,7 @@ class KvCache:
             ld = pos_ld
         lengths = torch.empty_like(starts)           # (quicker than torch.empty)
         self._check(self.lib.taco_kv_append(
-            self._ref, table.data_ptr(), table.stride(0), B, max_pages,
+            self._ref, table.data_ptr(), table_ld, B, max_pages,
             k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], T,
             starts.data_ptr(), counts.data_ptr() if counts is not None else None,
             first.data_ptr() if first is not None else None, mass.data_ptr() if mass is not None else None,
@@ -174,8 +180,8 @@ class KvCache:
         if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.shape[2] != self.head_dim or not q.numel():
             raise TacoError('q must be [B, q_heads, %d]' % self.head_dim)
         B, hq, _ = q.shape
-        (q, qs), table = self._rows(q, 'q'), self._table(page_table, B)
-        max_pages = table.shape[1]
+        q, qs = self._rows(q, 'q')
+        table, table_ld, _, max_pages = self._table(page_table, B)
         lengths = self._ints(lengths, 'lengths', B)
         ld = 0
         if mass is not None:
@@ -184,7 +190,7 @@ class KvCache:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((B, hq), dtype=torch.float32, device=self.device)
         self._check(self.lib.taco_kv_attend(
-            self._ref, table.data_ptr(), table.stride(0), B, max_pages, lengths.data_ptr(), q.data_ptr(), qs[0],
+            self._ref, table.data_ptr(), table_ld, B, max_pages, lengths.data_ptr(), q.data_ptr(), qs[0],
             qs[1], hq, 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), out.data_ptr(),
             lse.data_ptr(), mass.data_ptr() if mass is not None else None, ld, ws.data_ptr(), need, self._stream()))
         return out, lse
@@ -195,8 +201,7 @@ class KvCache:
         slots end up in no order; `positions` tells which token a slot holds. Returns (lengths, mass, positions), new
         tensors, or `out` = three tensors to write, each of which may be the matching input itself. Slots from the new
         length on get mass 0 and position -1 and their pages may be given away. The pages must belong to one sequence."""
-        table = self._table(page_table)
-        B, max_pages = table.shape
+        table, table_ld, B, max_pages = self._table(page_table)
         lengths = self._ints(lengths, 'lengths', B)
         slots = max_pages * self.page_size
         ld = self._side(mass, 'mass', torch.float32, B, slots)
@@ -217,7 +222,7 @@ class KvCache:
                     raise TacoError('%s must have the shape of its input' % name)
         ws, need = self._workspace('taco_kv_evict_workspace_bytes', B, max_pages, budget)
         self._check(self.lib.taco_kv_evict(
-            self._ref, table.data_ptr(), table.stride(0), B, max_pages, lengths.data_ptr(), mass.data_ptr(),
+            self._ref, table.data_ptr(), table_ld, B, max_pages, lengths.data_ptr(), mass.data_ptr(),
             positions.data_ptr(), ld, budget, recent, new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr(),
             ws.data_ptr(), need, self._stream()))
         return new
