@@ -43,7 +43,7 @@ class KvCache:
         self.device, self.dtype, self._index = k_pages.device, k_pages.dtype, k_pages.device.index
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
         own = torch.zeros(8, dtype=torch.int32, device=self.device)
-        self._status, self._none = own[:1], own[4:]  # _none: 16 bytes, the workspace of calls that use none
+        self._status, self._none = own[:1], own[4:]  # _none: 16 bytes, the workspace of attentions that use none
         p = _lib.TacoKvPool()
         p.struct_size = ctypes.sizeof(p)
         p.device, p.dtype = self.device.index, _DTYPES[self.dtype]
@@ -130,7 +130,9 @@ class KvCache:
             if len(self._need) >= 256:
                 self._need.clear()
             self._need[(query, sizes)] = need
-        if need <= 16:                               # the least there is
+        # The one buffer that calls share is for those that leave it alone: an attention that is said to need the least there
+        # is. (An eviction of one head to one token uses all of its 16 bytes.)
+        if need <= 16 and query == 'taco_kv_attend_workspace_bytes':
             return self._none, need
         return torch.empty(need, dtype=torch.uint8, device=self.device), need
 

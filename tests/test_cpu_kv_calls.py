@@ -1,0 +1,38 @@
+"""What the key-value cache's calls share and refuse, without a GPU: workspaces, aliases and the variant builds of its source."""
+import ctypes
+
+from tests.test_cpu_kv_cache import _pool
+
+
+def _host_cache(**pool):
+    """A KvCache on the host whose buffers are never touched by a kernel: for the parts of a call before its launch."""
+    import torch
+    from tacotron_amd import _lib
+    from tacotron_amd.kv_cache import KvCache
+    c = object.__new__(KvCache)
+    c.lib, c._need, c._none, c.device = _lib.load_library(), {}, torch.zeros(4, dtype=torch.int32), torch.device('cpu')
+    c._pool = _pool(**pool)
+    c._ref = ctypes.byref(c._pool)
+    return c
+
+
+def test_every_eviction_has_a_workspace_of_its_own():
+    """The smallest one too: a sequence, one kv head and a budget of 1 need 16 bytes, two counts and an entry of each list."""
+    c = _host_cache(kv_heads=1)
+    for max_pages, budget in ((4, 1), (1024, 1), (4, 2), (2048, 1)):
+        a, b = (c._workspace('taco_kv_evict_workspace_bytes', 1, max_pages, budget) for _ in range(2))
+        assert a[1] == b[1] and a[0].numel() * a[0].element_size() >= a[1]
+        assert len({a[0].data_ptr(), b[0].data_ptr(), c._none.data_ptr()}) == 3
+    assert c._workspace('taco_kv_evict_workspace_bytes', 1, 4, 1)[1] == 16
+
+
+def test_attention_of_a_short_memory_uses_no_workspace():
+    """Where the buffer that all calls may be given stands for "none": the library asks for the least there is only where the
+    kernel takes none, and for more wherever it takes one."""
+    c = _host_cache(kv_heads=1)
+    ws, need = c._workspace('taco_kv_attend_workspace_bytes', 1, 1, 4, True)
+    assert ws is c._none and need == 16 == ws.numel() * ws.element_size()
+    for dim, max_pages in ((64, 64), (128, 64), (256, 1), (256, 4)):
+        c = _host_cache(kv_heads=1, head_dim=dim)
+        (a, need), (b, _) = (c._workspace('taco_kv_attend_workspace_bytes', 1, 1, max_pages, False) for _ in range(2))
+        assert need > 16 and len({a.data_ptr(), b.data_ptr(), c._none.data_ptr()}) == 3
