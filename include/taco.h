@@ -309,7 +309,7 @@ typedef struct TacoKvPool {
  *   k, v [B, T, kv_heads, head_dim]: strides of batch, token, head
  *   mass [B, kv_heads, side_ld] fp32, or NULL: 0 for the new slots
  *   positions [B, kv_heads, side_ld] int32, or NULL: first[b] + t (first NULL = starts) for the new slots
- *   lengths_out [B] int32: starts[b] + counts[b]
+ *   lengths_out [B] int32: starts[b] + counts[b]. Not in place: a buffer apart from starts, counts and first (else refused)
  * side_ld >= max_pages * page_size. Tokens beyond the table's capacity are dropped (TACO_KV_BAD_LENGTH). The pages that
  * are written must be the sequence's own, and k and v no part of the pool. */
 int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,

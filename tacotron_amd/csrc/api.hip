@@ -1719,6 +1719,11 @@ int kv_rows(const char* what, const KvPool& p, const void* x, const int64_t* st,
     return 0;
 }
 
+// Whether the ranges [a, a + an) and [b, b + bn) have a byte in common.
+bool ranges_meet(const void* a, size_t an, const void* b, size_t bn) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+
 }  // namespace
 
 extern "C" int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
@@ -1739,6 +1744,10 @@ extern "C" int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int6
     if (!starts || !lengths_out) return fail("%s: null argument", what);
     if (mass || positions)
         if (int rc = kv_side(what, p, t, side_ld)) return rc;
+    // one workgroup of a sequence writes its length while others have yet to read where it starts
+    const size_t ints = (size_t)B * sizeof(int32_t);
+    for (const int32_t* in : {starts, counts, first})
+        if (ranges_meet(lengths_out, ints, in, ints)) return fail("%s: lengths_out must not overlap starts, counts or first", what);
     DeviceScope scope(pool->device);
     if (!scope.ok) return fail("%s: device %d is not available", what, pool->device);
     launch_kv_append(p, t, a, (hipStream_t)stream);

@@ -1,7 +1,11 @@
 """What the key-value cache's calls share and refuse, without a GPU: workspaces, aliases and the variant builds of its source."""
 import ctypes
 
-from tests.test_cpu_kv_cache import _pool
+import pytest
+
+from tests.test_cpu_kv_cache import _append, _pool
+
+NOWHERE = 1000      # a device that no machine has: a call that is not refused before ends there, and launches nothing
 
 
 def _host_cache(**pool):
@@ -36,3 +40,21 @@ def test_attention_of_a_short_memory_uses_no_workspace():
         c = _host_cache(kv_heads=1, head_dim=dim)
         (a, need), (b, _) = (c._workspace('taco_kv_attend_workspace_bytes', 1, 1, max_pages, False) for _ in range(2))
         assert need > 16 and len({a.data_ptr(), b.data_ptr(), c._none.data_ptr()}) == 3
+
+
+@pytest.mark.parametrize('which', ['starts', 'counts', 'first'])
+@pytest.mark.parametrize('shift,refused', [(0, True), (4, True), (-12, True), (16, False), (-16, False)])
+def test_append_refuses_to_write_lengths_over_what_it_reads(which, shift, refused):
+    """A launch's workgroups read starts, counts and first while one of them writes the new lengths."""
+    from tacotron_amd import _lib
+    at = dict(starts=1 << 16, counts=2 << 16, first=3 << 16)
+    args = dict(at, B=4, k=16, v=16, lengths=at[which] + shift)
+    assert _append(_lib.load_library(), _pool(device=NOWHERE), **args) < 0
+    assert ('lengths_out' if refused else 'device') in _lib.last_error(), _lib.last_error()
+
+
+def test_append_without_counts_and_firsts():
+    from tacotron_amd import _lib
+    lib = _lib.load_library()
+    assert _append(lib, _pool(device=NOWHERE), starts=1 << 16, lengths=2 << 16) < 0 and 'device' in _lib.last_error()
+    assert _append(lib, _pool(device=NOWHERE), starts=1 << 16, lengths=1 << 16) < 0 and 'lengths_out' in _lib.last_error()
