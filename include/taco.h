@@ -322,8 +322,8 @@ int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_l
  *   lse[b][h] = log sum_t exp s[h][t],   out[b][h] = sum_t exp(s[h][t] - lse[b][h]) v[b][h / group][t],
  *   mass[b][j][t] += sum over the `group` query heads h of kv head j of exp(s[h][t] - lse[b][h])      (mass not NULL)
  * q [B, q_heads, head_dim] by strides of batch and head, q_heads = group * kv_heads; out [B, q_heads, head_dim] and
- * lse [B, q_heads] (fp32, natural log) contiguous; mass [B, kv_heads, side_ld] fp32. Pages may be shared between
- * sequences. A row without tokens, or whose scores are all -inf, gives out 0 and lse -inf and leaves its mass alone.
+ * lse [B, q_heads] (fp32, natural log) contiguous and apart from all that is read, but out may be q itself where that is
+ * contiguous (another overlap with q is refused); mass [B, kv_heads, side_ld] fp32. Pages may be shared between sequences. A row without tokens, or whose scores are all -inf, gives out 0 and lse -inf and leaves its mass alone.
  * What masked slots and unused pages hold (NaN, infinities) has no influence; a NaN or an infinity among a row's own tokens
  * makes that row's output NaN or infinite and no other. Sums and softmax statistics are fp32. The same call gives the same
  * bits; how a row's sums are cut depends on the batch and all its lengths, so a row's last bits may differ in another. Short

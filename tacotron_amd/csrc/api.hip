@@ -1724,6 +1724,15 @@ bool ranges_meet(const void* a, size_t an, const void* b, size_t bn) {
     return a && b && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
 }
 
+// Whether x meets the rows of a sequence's queries (of all heads and what lies between them), for any sequence.
+bool meets_queries(const void* x, size_t n, const KvPool& p, const KvAttend& a, int B) {
+    const size_t one = ((size_t)(p.heads * a.group - 1) * a.q_st[1] + p.dim) * p.esize, step = (size_t)a.q_st[0] * p.esize;
+    if (!ranges_meet(x, n, a.q, (B - 1) * step + one)) return false;
+    for (int b = 0; b < B; ++b)
+        if (ranges_meet(x, n, (const char*)a.q + b * step, one)) return true;
+    return false;
+}
+
 }  // namespace
 
 extern "C" int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
@@ -1782,6 +1791,12 @@ extern "C" int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int6
         if (int rc = kv_side(what, p, t, side_ld)) return rc;
     if (!ws || !aligned16(ws) || ws_bytes < kv_attend_ws_bytes(p, B, a.group, max_pages, mass != nullptr))
         return fail("%s: workspace too small (taco_kv_attend_workspace_bytes) or not on a 16-byte boundary", what);
+    // Queries are read as a wave comes to their head, when other heads may be written already. A head's own row is written by
+    // who read it, or after all have: contiguous queries may be written over in place.
+    const size_t heads = (size_t)B * q_heads;
+    const bool in_place = out == q && a.q_st[1] == p.dim && (B == 1 || a.q_st[0] == (int64_t)q_heads * p.dim);
+    if ((!in_place && meets_queries(out, heads * p.dim * p.esize, p, a, B)) || meets_queries(lse, heads * sizeof(float), p, a, B))
+        return fail("%s: out must be the (contiguous) queries or not overlap them, nor may lse", what);
     DeviceScope scope(pool->device);
     if (!scope.ok) return fail("%s: device %d is not available", what, pool->device);
     launch_kv_attend(p, t, a, ws, (hipStream_t)stream);

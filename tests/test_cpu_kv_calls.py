@@ -3,7 +3,7 @@ import ctypes
 
 import pytest
 
-from tests.test_cpu_kv_cache import _append, _pool
+from tests.test_cpu_kv_cache import _append, _attend, _pool
 
 NOWHERE = 1000      # a device that no machine has: a call that is not refused before ends there, and launches nothing
 
@@ -58,3 +58,39 @@ def test_append_without_counts_and_firsts():
     lib = _lib.load_library()
     assert _append(lib, _pool(device=NOWHERE), starts=1 << 16, lengths=2 << 16) < 0 and 'device' in _lib.last_error()
     assert _append(lib, _pool(device=NOWHERE), starts=1 << 16, lengths=1 << 16) < 0 and 'lengths_out' in _lib.last_error()
+
+
+@pytest.mark.parametrize('out,lse,refused', [
+    (0, None, True), (-256, None, True), (1536 + 16, None, True),                # over the queries of the first or last sequence
+    (528, None, True), (512, None, False),                                       # the gap between them holds it just so
+    (-1024, None, False), (1536 + 512, None, False),                             # before and behind them all
+    (None, 0, True), (None, 512, False), (None, 1536 + 508, True)])              # lse: on a query, in a gap, on the last of them
+def test_attend_refuses_to_write_over_its_queries(out, lse, refused):
+    """Queries [2, 2, 64] fp32, 1536 bytes from one sequence's to the next's (512 bytes each): waves read them as they come to
+    a head, when others may have written theirs."""
+    from tacotron_amd import _lib
+    q = 1 << 20
+    args = dict(B=2, q=q, qs=(384, 64), out=(1 << 21) if out is None else q + out, lse=(1 << 22) if lse is None else q + lse)
+    assert _attend(_lib.load_library(), _pool(device=NOWHERE), **args) < 0
+    assert ('overlap' if refused else 'device') in _lib.last_error(), _lib.last_error()
+
+
+@pytest.mark.parametrize('B,qs,refused', [(2, (128, 64), False), (1, (384, 64), False), (2, (384, 64), True), (1, (128, 128), True)])
+def test_attend_in_place_takes_contiguous_queries(B, qs, refused):
+    from tacotron_amd import _lib
+    q = 1 << 20
+    assert _attend(_lib.load_library(), _pool(device=NOWHERE), B=B, q=q, qs=qs, out=q, lse=1 << 22) < 0
+    assert ('overlap' if refused else 'device') in _lib.last_error(), _lib.last_error()
+
+
+@pytest.mark.parametrize('kw', [dict(), dict(head_dim=256), dict(dtype=1), dict(head_dim=128, dtype=2)])
+@pytest.mark.parametrize('with_mass', [0, 1])
+def test_attend_refuses_a_workspace_one_byte_short(kw, with_mass):
+    """Tables past what the kernel without a workspace takes."""
+    from tacotron_amd import _lib
+    lib, p = _lib.load_library(), _pool(device=NOWHERE, **kw)
+    args = dict(B=3, table_ld=400, max_pages=400, qs=(1024, 256), q=1 << 16, out=1 << 20, lse=1 << 24, mass=(1 << 28) if with_mass else None, side_ld=6400)
+    need = lib.taco_kv_attend_workspace_bytes(ctypes.byref(p), 3, 2, 400, with_mass)
+    assert need > 16
+    assert _attend(lib, p, ws_bytes=need - 1, **args) < 0 and 'workspace' in _lib.last_error()
+    assert _attend(lib, p, ws_bytes=need, **args) < 0 and 'device' in _lib.last_error()

@@ -2,7 +2,7 @@
 cache object itself keeps."""
 import pytest
 
-from tests.test_gpu_kv_cache import _make
+from tests.test_gpu_kv_cache import TYPES, _make, _q
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,21 @@ def test_captured_evictions_beside_eager_ones(slots, budget):
         assert all(_same(a, b) for a, b in zip(e.outcome(results), want)), turn
         torch.zeros(1 << 20, device='cuda').add_(1)
     e.cache.status()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('d,hkv,group,lens', [
+    (64, 2, 3, [40, 0, 64, 1]), (128, 1, 16, [100, 7]), (256, 3, 17, [33, 150, 2]), (64, 1, 40, [9000, 0, 5]), (128, 2, 4, [20000])])
+def test_attend_over_its_queries(dtype, d, hkv, group, lens):
+    """The C entry with contiguous queries as the output too: the bits of a call with a buffer of its own."""
+    import torch
+    from tacotron_amd import _lib
+    cache, table, lengths = _make(d + group, lens, hkv, d, 16, dtype)
+    B, hq, mp, lib = len(lens), hkv * group, table.shape[1], _lib.load_library()
+    q = _q(group, B, hq, d, dtype)
+    want, want_lse = cache.attend(q, table, lengths)
+    lse = torch.empty_like(want_lse)
+    ws = torch.empty(lib.taco_kv_attend_workspace_bytes(cache._ref, B, hq, mp, 0), dtype=torch.uint8, device='cuda')
+    assert lib.taco_kv_attend(cache._ref, table.data_ptr(), mp, B, mp, lengths.data_ptr(), q.data_ptr(), hq * d, d, hq, d ** -0.5, q.data_ptr(),
+                              lse.data_ptr(), None, 0, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
+    assert _same(q, want) and _same(lse, want_lse)
