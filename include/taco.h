@@ -303,6 +303,10 @@ typedef struct TacoKvPool {
     int32_t* status;              /* device int32[1], zeroed by the caller: TACO_KV_BAD_* bits are or-ed into it */
 } TacoKvPool;
 
+/* *bits (device int32[1]) = *status, and *status = 0, in one step: what calls of other streams meet meanwhile is in *bits or
+ * stays in *status, and is not lost. */
+int taco_kv_take_status(const TacoKvPool* pool, int32_t* bits, taco_stream_t stream);
+
 /* Rows into pages: token t < counts[b] of sequence b goes to slot starts[b] + t, that is row slot % page_size of page
  * table[b][slot / page_size]; tokens from counts[b] on, and pages of no token, stay untouched.
  *   table [B, max_pages] int32, rows table_ld apart; starts, counts, first [B] int32 (counts NULL = T each)

@@ -44,7 +44,7 @@ class TacoKvPool(ctypes.Structure):
 EXPORTS = ['taco_last_error', 'taco_create', 'taco_destroy', 'taco_workspace_bytes', 'taco_encode',
            'taco_decode', 'taco_decode_teacher', 'taco_postnet', 'taco_griffin_lim', 'taco_griffin_lim_noalloc', 'taco_griffin_lim_librosa', 'taco_spectrogram', 'taco_spectrogram_workspace_bytes', 'taco_synthesize', 'taco_timing_begin',
            'taco_timing_end', 'taco_kernel_name', 'taco_num_kernel_kinds', 'taco_set_decode_graph', 'taco_set_persist_budget', 'taco_get_persist_budget', 'taco_set_gl_split', 'taco_set_bigru_mode', 'taco_decode_status', 'taco_debug_conv_gemm', 'taco_debug_handoff_probe',
-           'taco_debug_poison_decoder', 'taco_kv_append', 'taco_kv_attend', 'taco_kv_attend_workspace_bytes',
+           'taco_debug_poison_decoder', 'taco_kv_take_status', 'taco_kv_append', 'taco_kv_attend', 'taco_kv_attend_workspace_bytes',
            'taco_kv_evict', 'taco_kv_evict_workspace_bytes']
 
 _lib = None
@@ -118,6 +118,8 @@ def load_library():
     lib.taco_debug_conv_gemm.restype = ctypes.c_int
     lib.taco_debug_conv_gemm.argtypes = [vp, i32, i32, i32, i32, i32, i32, vp, i32, i32, vp, vp, vp, vp, i32, vp, i32, i32, i32, vp]
     i64, pool = ctypes.c_int64, ctypes.POINTER(TacoKvPool)
+    lib.taco_kv_take_status.restype = ctypes.c_int
+    lib.taco_kv_take_status.argtypes = [pool, vp, vp]
     lib.taco_kv_append.restype = ctypes.c_int
     lib.taco_kv_append.argtypes = [pool, vp, i64, i32, i32, vp, i64, i64, i64, vp, i64, i64, i64, i32, vp, vp, vp, vp, vp,
                                    i64, vp, vp]

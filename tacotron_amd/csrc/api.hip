@@ -1735,6 +1735,17 @@ bool meets_queries(const void* x, size_t n, const KvPool& p, const KvAttend& a, 
 
 }  // namespace
 
+extern "C" int taco_kv_take_status(const TacoKvPool* pool, int32_t* bits, taco_stream_t stream) {
+    const char* what = "taco_kv_take_status";
+    KvPool p;
+    if (int rc = kv_pool_view(what, pool, &p)) return rc;
+    if (!bits) return fail("%s: null argument", what);
+    DeviceScope scope(pool->device);
+    if (!scope.ok) return fail("%s: device %d is not available", what, pool->device);
+    launch_kv_take_status(p.status, bits, (hipStream_t)stream);
+    return check_launch(what);
+}
+
 extern "C" int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
                               const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
                               const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,

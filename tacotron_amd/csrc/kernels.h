@@ -284,6 +284,7 @@ struct KvEvict {
     int32_t* counts; int32_t* lists; int64_t list_ld;      // workspace, as the next line
     int32_t* chunk_newest; uint32_t* chunk_hist; uint32_t* chunk_list;
 };
+void launch_kv_take_status(int32_t* status, int32_t* bits, hipStream_t s);
 void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hipStream_t s);
 bool kv_attend_fits(const KvPool& p, int B, int group, int max_pages);
 size_t kv_attend_ws_bytes(const KvPool& p, int B, int group, int max_pages, bool mass);

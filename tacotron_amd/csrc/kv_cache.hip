@@ -39,6 +39,8 @@ __device__ __forceinline__ int64_t slot_off(const int64_t* st, int page, int h, 
     return (int64_t)page * st[0] + (int64_t)h * st[1] + (int64_t)in_page * st[2];
 }
 
+__global__ void kv_take_status_kernel(int32_t* status, int32_t* bits) { *bits = atomicExch(status, 0); }
+
 // ---------------------------------------------------------------------------------------
 // append
 
@@ -1395,6 +1397,8 @@ static int kv_cus(int device) {
     known[device].store(n, std::memory_order_relaxed);
     return n;
 }
+
+void launch_kv_take_status(int32_t* status, int32_t* bits, hipStream_t s) { kv_take_status_kernel<<<1, 1, 0, s>>>(status, bits); }
 
 void launch_kv_append(const KvPool& p, const KvTable& tb, const KvAppend& a, hipStream_t s) {
     const int64_t pieces = (int64_t)a.T * p.heads * ((p.dim * p.esize) >> 4);

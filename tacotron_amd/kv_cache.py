@@ -69,9 +69,10 @@ class KvCache:
         """Synchronises the device; raises TacoError if any call since the last status() met a length outside its table's
         capacity or a page id outside the pool (which it treated as masked)."""
         torch.cuda.synchronize(self.device)
-        bits = int(self._status.item())
+        taken = torch.empty_like(self._status)
+        self._check(self.lib.taco_kv_take_status(self._ref, taken.data_ptr(), self._stream()))
+        bits = int(taken.item())
         if bits:
-            self._status.zero_()
             raise TacoError('KvCache: ' + ', '.join(m for b, m in ((1, 'a page id outside the pool'),
                                                                   (2, "a length outside the page table's capacity"))
                                                     if bits & b))

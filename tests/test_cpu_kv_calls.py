@@ -94,3 +94,13 @@ def test_attend_refuses_a_workspace_one_byte_short(kw, with_mass):
     assert need > 16
     assert _attend(lib, p, ws_bytes=need - 1, **args) < 0 and 'workspace' in _lib.last_error()
     assert _attend(lib, p, ws_bytes=need, **args) < 0 and 'device' in _lib.last_error()
+
+
+def test_take_status_refusals():
+    from tacotron_amd import _lib
+    lib = _lib.load_library()
+    p = _pool(device=NOWHERE)
+    assert lib.taco_kv_take_status(None, 16, None) < 0 and 'null' in _lib.last_error()
+    assert lib.taco_kv_take_status(ctypes.byref(p), None, None) < 0 and 'null' in _lib.last_error()
+    assert lib.taco_kv_take_status(ctypes.byref(_pool(status=None)), 16, None) < 0 and 'null' in _lib.last_error()
+    assert lib.taco_kv_take_status(ctypes.byref(p), 16, None) < 0 and 'device' in _lib.last_error()

@@ -104,3 +104,36 @@ def test_attend_over_its_queries(dtype, d, hkv, group, lens):
     assert lib.taco_kv_attend(cache._ref, table.data_ptr(), mp, B, mp, lengths.data_ptr(), q.data_ptr(), hq * d, d, hq, d ** -0.5, q.data_ptr(),
                               lse.data_ptr(), None, 0, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
     assert _same(q, want) and _same(lse, want_lse)
+
+
+def _one_bad_page():
+    """A call that meets a page id outside the pool, and a cache to make it with."""
+    import torch
+    cache, table, lengths = _make(5, [40], 1, 64, 16, 'float32')
+    bad = table.clone()
+    bad[0, 1] = cache.num_pages
+    q = _q(1, 1, 2, 64, 'float32')
+    torch.cuda.synchronize()
+    return cache, bad, lengths, q
+
+
+def test_status_keeps_what_is_met_while_it_is_read(monkeypatch):
+    """A call of another stream between the reading of the word and its clearing."""
+    import torch
+    from tacotron_amd.engine import TacoError
+    cache, bad, lengths, q = _one_bad_page()
+    side, read = torch.cuda.Stream(), torch.Tensor.item
+
+    def item(t):
+        x = read(t)
+        monkeypatch.undo()
+        with torch.cuda.stream(side):
+            cache.attend(q, bad, lengths)
+        torch.cuda.synchronize()
+        return x
+    cache.attend(q, bad, lengths)
+    monkeypatch.setattr(torch.Tensor, 'item', item)
+    for _ in range(2):
+        with pytest.raises(TacoError, match='page id'):
+            cache.status()
+    cache.status()
