@@ -43,6 +43,9 @@ class KvCache:
         self.device, self.dtype, self._index = k_pages.device, k_pages.dtype, k_pages.device.index
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
         own = torch.zeros(8, dtype=torch.int32, device=self.device)
+        with torch.cuda.device(self.device):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()      # zeroed before a call of any stream may set a bit
         self._status, self._none = own[:1], own[4:]  # _none: 16 bytes, the workspace of attentions that use none
         p = _lib.TacoKvPool()
         p.struct_size = ctypes.sizeof(p)

@@ -137,3 +137,18 @@ def test_status_keeps_what_is_met_while_it_is_read(monkeypatch):
         with pytest.raises(TacoError, match='page id'):
             cache.status()
     cache.status()
+
+
+def test_status_of_a_cache_made_on_a_busy_stream():
+    """What a call of another stream meets before the stream of the cache's making has come so far."""
+    import torch
+    from tacotron_amd.engine import TacoError
+    from tacotron_amd.kv_cache import KvCache
+    made, bad, lengths, q = _one_bad_page()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda._sleep(50_000_000)
+        cache = KvCache(made.k_pages, made.v_pages)
+    cache.attend(q, bad, lengths)
+    with pytest.raises(TacoError, match='page id'):
+        cache.status()
+    cache.status()
