@@ -8,7 +8,8 @@ collected `mass` being the alignments summed over the steps.
 The cache object holds the pool's geometry and a status word. Everything else - page tables, lengths, masses, positions -
 is the caller's and is passed to each call, so one pool serves any number of batches and a captured HIP graph follows what
 the tensors hold when it runs. Calls are queued on torch's current stream of the pool's device and synchronise nothing;
-workspaces and results come from torch's allocator, so calls on several streams do not share any. A serving form: no
+workspaces and results come from torch's allocator, so calls on several streams do not share any. A captured graph holds the
+addresses of the pool and of the status word: the cache has to live as long as it is replayed. A serving form: no
 gradients are recorded."""
 import ctypes
 import math
@@ -43,6 +44,7 @@ class KvCache:
         self.device, self.dtype, self._index = k_pages.device, k_pages.dtype, k_pages.device.index
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
         own = torch.zeros(8, dtype=torch.int32, device=self.device)
+        self._own, self._streams = own, {self._raw_stream()}
         with torch.cuda.device(self.device):
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream().synchronize()      # zeroed before a call of any stream may set a bit
@@ -140,9 +142,19 @@ class KvCache:
             return self._none, need
         return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
-    def _stream(self):
+    def _raw_stream(self):
         # the handle alone: torch.cuda.current_stream builds an object around it
         return torch._C._cuda_getCurrentRawStream(self._index)
+
+    def _stream(self):
+        """The stream a call is queued on. The cache holds the status word and the pool: torch's allocator is told of every
+        stream that calls ran on, so that it waits for them before it gives that memory to other tensors."""
+        s = self._raw_stream()
+        if s not in self._streams:
+            for t in (self._own, self.k_pages, self.v_pages):
+                t.record_stream(torch.cuda.current_stream(self.device))
+            self._streams.add(s)
+        return s
 
     # ---- the operators
     def append(self, k, v, page_table, starts, counts=None, first=None, mass=None, positions=None):

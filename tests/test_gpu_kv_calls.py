@@ -152,3 +152,23 @@ def test_status_of_a_cache_made_on_a_busy_stream():
     with pytest.raises(TacoError, match='page id'):
         cache.status()
     cache.status()
+
+
+def test_a_cache_that_goes_while_a_call_runs():
+    """Neither the status word nor the pool is given to another tensor before the calls of every stream are over."""
+    import torch
+    from tacotron_amd.kv_cache import KvCache
+    table = torch.zeros(1, 3, dtype=torch.int32, device='cuda')
+    lengths = torch.full((1,), 40, dtype=torch.int32, device='cuda')
+    q = _q(1, 1, 2, 64, 'float32')
+    side = torch.cuda.Stream()
+    cache = KvCache.empty(1024, 16, 1, 64)
+    held = {x.data_ptr() for x in (cache._status, cache.k_pages, cache.v_pages)}
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        out, lse = cache.attend(q, table, lengths)
+    del cache
+    others = [torch.empty(n, dtype=torch.int32, device='cuda') for n in [8] * 200 + [1 << 20] * 4]
+    assert not side.query() and not held & {x.data_ptr() for x in others}
+    torch.cuda.synchronize()
