@@ -1636,14 +1636,16 @@ extern "C" int taco_debug_conv_gemm(const float* X, int32_t ldx, int32_t M, int3
 // paged key-value cache
 namespace {
 
-// The call's device for its launches; the thread's current device again afterwards.
+// The call's device for its launches; the thread's current device again afterwards. (Where there is no such device the call is
+// refused: HIP's last error is cleared, or the next call would report it.)
 struct DeviceScope {
     int prev = -1;
     bool ok = true;
     explicit DeviceScope(int device) {
-        if (hipGetDevice(&prev) != hipSuccess) { ok = false; prev = -1; return; }
-        if (prev == device) prev = -1;
+        if (hipGetDevice(&prev) != hipSuccess) { ok = false; prev = -1; }
+        else if (prev == device) prev = -1;
         else ok = hipSetDevice(device) == hipSuccess;
+        if (!ok) (void)hipGetLastError();
     }
     ~DeviceScope() { if (prev >= 0) (void)hipSetDevice(prev); }
 };

@@ -172,3 +172,23 @@ def test_a_cache_that_goes_while_a_call_runs():
     others = [torch.empty(n, dtype=torch.int32, device='cuda') for n in [8] * 200 + [1 << 20] * 4]
     assert not side.query() and not held & {x.data_ptr() for x in others}
     torch.cuda.synchronize()
+
+
+def test_a_call_for_no_device_leaves_no_error_behind():
+    """What is refused for its device is not reported again by the next call, nor by the library's next launch."""
+    import ctypes
+
+    import torch
+    from tacotron_amd import _lib
+    cache, table, lengths = _make(6, [40], 1, 64, 16, 'float32')
+    q = _q(1, 1, 2, 64, 'float32')
+    want, _ = cache.attend(q, table, lengths)
+    pool = type(cache._pool).from_buffer_copy(cache._pool)
+    pool.device = torch.cuda.device_count()
+    bits = torch.zeros(1, dtype=torch.int32, device='cuda')
+    torch.cuda.synchronize()
+    assert cache.lib.taco_kv_take_status(ctypes.byref(pool), bits.data_ptr(), None) < 0 and 'not available' in _lib.last_error()
+    got, _ = cache.attend(q, table, lengths)
+    assert torch.equal(got, want)
+    assert cache.lib.taco_kv_take_status(ctypes.byref(pool), bits.data_ptr(), None) < 0
+    assert (bits + 1).item() == 1
