@@ -10,7 +10,7 @@ is the caller's and is passed to each call, so one pool serves any number of bat
 the tensors hold when it runs. Calls are queued on torch's current stream of the pool's device and synchronise nothing;
 workspaces and results come from torch's allocator, so calls on several streams do not share any. A captured graph holds the
 addresses of the pool and of the status word: the cache has to live as long as it is replayed. A serving form: no
-gradients are recorded."""
+gradients are recorded, and tensors that require one are refused while gradients are."""
 import ctypes
 import math
 
@@ -35,6 +35,7 @@ class KvCache:
                 raise TacoError('%s: rows of head_dim must be contiguous' % name)
             if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
                 raise TacoError('%s: an expanded tensor cannot be a pool' % name)
+            self._no_gradient(t, name)
         if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device:
             raise TacoError('k_pages and v_pages must agree in shape, type and device')
         if k_pages.device.type != 'cuda':
@@ -87,6 +88,10 @@ class KvCache:
         if rc != 0:
             raise TacoError(_lib.last_error())
 
+    def _no_gradient(self, t, name):
+        if t.requires_grad and torch.is_grad_enabled():
+            raise TacoError('%s requires a gradient, and KvCache records none: pass it detached or call under torch.no_grad()' % name)
+
     # (get_device, an int, is -1 for host tensors; comparing devices builds objects)
     def _ints(self, t, name, B):
         if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != self._index or t.shape != (B,):
@@ -107,6 +112,7 @@ class KvCache:
 
     def _side(self, t, name, dtype, B, slots):
         if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self._index and t.dim() == 3 and t.is_contiguous():
+            self._no_gradient(t, name)
             n, h, ld = t.shape
             if n == B and h == self.kv_heads and ld >= slots:
                 return ld
@@ -117,6 +123,7 @@ class KvCache:
         """Rows of head_dim elements: contiguous, 16-byte aligned, or copied to be. Returns it and its strides."""
         if t.dtype is not self.dtype or t.get_device() != self._index:
             raise TacoError('%s must be %s on %s, as the pool' % (name, str(self.dtype)[6:], self.device))
+        self._no_gradient(t, name)
         st = t.stride()
         bits = t.data_ptr()
         for s in st[:-1]:

@@ -104,3 +104,30 @@ def test_take_status_refusals():
     assert lib.taco_kv_take_status(ctypes.byref(p), None, None) < 0 and 'null' in _lib.last_error()
     assert lib.taco_kv_take_status(ctypes.byref(_pool(status=None)), 16, None) < 0 and 'null' in _lib.last_error()
     assert lib.taco_kv_take_status(ctypes.byref(p), 16, None) < 0 and 'device' in _lib.last_error()
+
+
+def test_gradients_are_refused_and_not_dropped():
+    """A serving form: what would need a gradient is an error while gradients are recorded, wherever it enters."""
+    import torch
+    from tacotron_amd.engine import TacoError
+    from tacotron_amd.kv_cache import KvCache
+    c = _host_cache()
+    c._index, c._esize, c.dtype, c.kv_heads = -1, 4, torch.float32, 2
+    for t in (torch.zeros(2, 6, 64), torch.zeros(2, 3, 2, 64), torch.zeros(2, 65, 64)[:, 1:]):
+        leaf = t.clone().requires_grad_()
+        for x in (leaf, leaf * 2, leaf[:, 1:]):
+            with pytest.raises(TacoError, match='gradient'):
+                c._rows(x, 'q')
+            with torch.no_grad():
+                c._rows(x, 'q')
+            c._rows(x.detach(), 'q')
+    mass = torch.zeros(1, 2, 64, requires_grad=True)
+    with pytest.raises(TacoError, match='gradient'):
+        c._side(mass, 'mass', torch.float32, 1, 64)
+    with torch.no_grad():
+        assert c._side(mass, 'mass', torch.float32, 1, 64) == 64
+    assert c._side(mass.detach(), 'mass', torch.float32, 1, 64) == 64
+    pool = torch.zeros(4, 2, 16, 64)
+    for k, v in ((pool.clone().requires_grad_(), pool), (pool, pool.clone().requires_grad_())):
+        with pytest.raises(TacoError, match='gradient'):
+            KvCache(k, v)

@@ -192,3 +192,20 @@ def test_a_call_for_no_device_leaves_no_error_behind():
     assert torch.equal(got, want)
     assert cache.lib.taco_kv_take_status(ctypes.byref(pool), bits.data_ptr(), None) < 0
     assert (bits + 1).item() == 1
+
+
+def test_gradients_are_refused_by_the_calls():
+    import torch
+    from tacotron_amd.engine import TacoError
+    cache, table, lengths = _make(7, [40, 3], 1, 64, 16, 'float32')
+    q, rows = _q(1, 2, 2, 64, 'float32').requires_grad_(), torch.zeros(2, 1, 1, 64, device='cuda')
+    slots = table.shape[1] * 16
+    mass, pos = torch.zeros(2, 1, slots, device='cuda', requires_grad=True), torch.zeros(2, 1, slots, dtype=torch.int32, device='cuda')
+    for call in (lambda: cache.attend(q, table, lengths), lambda: cache.attend(q.detach(), table, lengths, mass=mass),
+                 lambda: cache.append(rows + q[:, None, :1], rows, table, lengths), lambda: cache.append(rows, rows + q[:, None, :1], table, lengths),
+                 lambda: cache.evict(table, lengths, mass, pos, 2), lambda: type(cache)(cache.k_pages.clone().requires_grad_(), cache.v_pages)):
+        with pytest.raises(TacoError, match='gradient'):
+            call()
+        with torch.no_grad():
+            call()
+    cache.status()
