@@ -1,7 +1,7 @@
 """Builds tacotron_amd/libtaco_hip.so (gfx950) from tacotron_amd/csrc/*.hip with hipcc.
 
 In-tree and explicit (no JIT cache): the shared object travels to the GPU box with the
-source snapshot. `python -m tacotron_amd.build [--force]`."""
+source snapshot. `python -m tacotron_amd.build [--force]`; `--flags <source.hip>` prints a source's compiler flags."""
 import os
 import subprocess
 import sys
@@ -28,6 +28,10 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def flags(src):
+    return FLAGS + EXTRA_FLAGS.get(src, [])
+
+
 def build(force=False, verbose=True):
     os.makedirs(OBJ, exist_ok=True)
     hdrs = [os.path.join(CSRC, h) for h in HEADERS]
@@ -35,11 +39,14 @@ def build(force=False, verbose=True):
     def compile_one(src):
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ, src.replace('.hip', '.o'))
-        if force or _stale(o, [s] + hdrs):
-            cmd = [HIPCC] + FLAGS + EXTRA_FLAGS.get(src, []) + ['-c', s, '-o', o]
+        cmd = [HIPCC] + flags(src) + ['-c', s, '-o', o]
+        made_by = o + '.cmd'                         # what the object there was compiled with
+        if force or _stale(o, [s] + hdrs) or not os.path.exists(made_by) or open(made_by).read() != ' '.join(cmd):
             if verbose:
                 print(' '.join(cmd), flush=True)
             subprocess.run(cmd, check=True)
+            with open(made_by, 'w') as f:
+                f.write(' '.join(cmd))
             return o, True
         return o, False
 
@@ -55,5 +62,8 @@ def build(force=False, verbose=True):
 
 
 if __name__ == '__main__':
-    build(force='--force' in sys.argv)
-    print(LIB)
+    if sys.argv[1:2] == ['--flags']:
+        print(' '.join(flags(sys.argv[2])))
+    else:
+        build(force='--force' in sys.argv)
+        print(LIB)
