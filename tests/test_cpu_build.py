@@ -53,3 +53,13 @@ def test_a_variant_build_keeps_the_flags_of_its_source(compiler, src, packed):
     assert all(f in compiled.split() for f in b.FLAGS + ['-DWHAT=1', '-c', 'tacotron_amd/csrc/' + src])
     assert ('-packed-fp32-ops' in compiled) == packed
     assert all(('/%s%s.o' % (s[:-4], '_test' if s == src else '')) in linked for s in b.SOURCES)
+
+
+def test_the_build_entry_compiles_whatever_is_there(monkeypatch):
+    """It is the check that the sources build, so an object from before is no reason to leave one out."""
+    import __graft_entry__ as g
+    from tacotron_amd import build as b
+    asked = []
+    monkeypatch.setattr(b, 'build', lambda force=False, verbose=True: asked.append(force) or b.LIB)
+    g.build()
+    assert asked == [True]
