@@ -209,3 +209,45 @@ def test_gradients_are_refused_by_the_calls():
         with torch.no_grad():
             call()
     cache.status()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('d', [64, 128, 256])
+@pytest.mark.parametrize('slots', [16, 3000])
+def test_attend_weights_keep_their_bits(dtype, d, slots):
+    """Three tokens of a sequence weigh w, 1 and 1, with values 1, -a and -b, where a + b is w to as many bits as two numbers of
+    the type hold: what is left, (w - a - b) / (2 + w), is there only if the weight's other bits reach the product.
+
+    Tolerance, in U = 2^-24 (half a step of fp32): the score is one product, exact, below 1 in units of ln 2; its factor and itself are
+    rounded (2 U, 1.4 in w), the exponential is off by a step (2 U), a sum of three products of at most 1 by up to 4 U, and a
+    weight in 16-bit pieces by half a step of the last: U / 2 (three of bf16), 4 U (two of fp16). Then the rounding to the type."""
+    import numpy as np
+    import torch
+    rng, U = np.random.default_rng(d), 2.0 ** -24
+    t = getattr(torch, dtype)
+    as_t = lambda x: torch.tensor(np.asarray(x)).to(t).double().numpy()  # noqa: E731
+    k, q = as_t(-rng.uniform(0.2, 0.9, 4000)), as_t(rng.uniform(0.2, 0.75, 4000))
+    w = np.exp(k * q)
+    a = as_t(w)
+    b = as_t(w - a)
+    left = w - a - b
+    if dtype == 'bfloat16':
+        pick = np.flatnonzero(np.abs(left) > 2.0 ** -18.5)
+        k, q, w, a, b, left = (x[pick] for x in (k, q, w, a, b, left))
+    k, q, w, a, b, left = (x[:64] for x in (k, q, w, a, b, left))
+    n = len(k)
+    assert n == 64
+    cache, table, lengths = _make(d, [3] * n, 1, d, 16, dtype, slots=slots)
+    rows = torch.zeros(2, n, 3, d, dtype=torch.float64)
+    rows[0, :, 0, 0] = torch.tensor(k)
+    rows[1, :, :, 5] = torch.tensor(np.stack([np.ones(n), -a, -b], 1))
+    for x, pages in zip(rows, (cache.k_pages, cache.v_pages)):
+        pages[table[:, 0].long(), 0, :3] = x.to(t).cuda()
+    qs = torch.zeros(n, 1, d, dtype=torch.float64)
+    qs[:, 0, 0] = torch.tensor(q)
+    out, _ = cache.attend(qs.to(t).cuda(), table, lengths, scale=1.0)
+    got, want = out[:, 0, 5].double().cpu().numpy(), left / (2 + w)
+    tol = ((1.4 + 2) * U * w + 4 * U + {'float32': 0, 'bfloat16': 0.5, 'float16': 4}[dtype] * U * w) / (2 + w)
+    tol += np.abs(want) * (torch.finfo(t).eps / 2 + 4 * U) + torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+    assert (out[:, 0, :5] == 0).all() and (out[:, 0, 6:] == 0).all()
