@@ -35,7 +35,8 @@ class KvCache:
                 raise TacoError('%s: rows of head_dim must be contiguous' % name)
             if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
                 raise TacoError('%s: an expanded tensor cannot be a pool' % name)
-            self._no_gradient(t, name)
+            if t.requires_grad:
+                self._no_gradient(name)
         if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device:
             raise TacoError('k_pages and v_pages must agree in shape, type and device')
         if k_pages.device.type != 'cuda':
@@ -45,7 +46,7 @@ class KvCache:
         self.device, self.dtype, self._index = k_pages.device, k_pages.dtype, k_pages.device.index
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
         own = torch.zeros(8, dtype=torch.int32, device=self.device)
-        self._own, self._streams = own, {self._raw_stream()}
+        self._own, self._streams = own, {torch._C._cuda_getCurrentRawStream(self._index)}
         with torch.cuda.device(self.device):
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream().synchronize()      # zeroed before a call of any stream may set a bit
@@ -88,8 +89,8 @@ class KvCache:
         if rc != 0:
             raise TacoError(_lib.last_error())
 
-    def _no_gradient(self, t, name):
-        if t.requires_grad and torch.is_grad_enabled():
+    def _no_gradient(self, name):
+        if torch.is_grad_enabled():
             raise TacoError('%s requires a gradient, and KvCache records none: pass it detached or call under torch.no_grad()' % name)
 
     # (get_device, an int, is -1 for host tensors; comparing devices builds objects)
@@ -112,7 +113,8 @@ class KvCache:
 
     def _side(self, t, name, dtype, B, slots):
         if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == self._index and t.dim() == 3 and t.is_contiguous():
-            self._no_gradient(t, name)
+            if t.requires_grad:
+                self._no_gradient(name)
             n, h, ld = t.shape
             if n == B and h == self.kv_heads and ld >= slots:
                 return ld
@@ -123,7 +125,8 @@ class KvCache:
         """Rows of head_dim elements: contiguous, 16-byte aligned, or copied to be. Returns it and its strides."""
         if t.dtype is not self.dtype or t.get_device() != self._index:
             raise TacoError('%s must be %s on %s, as the pool' % (name, str(self.dtype)[6:], self.device))
-        self._no_gradient(t, name)
+        if t.requires_grad:
+            self._no_gradient(name)
         st = t.stride()
         bits = t.data_ptr()
         for s in st[:-1]:
@@ -149,14 +152,11 @@ class KvCache:
             return self._none, need
         return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
-    def _raw_stream(self):
-        # the handle alone: torch.cuda.current_stream builds an object around it
-        return torch._C._cuda_getCurrentRawStream(self._index)
-
     def _stream(self):
         """The stream a call is queued on. The cache holds the status word and the pool: torch's allocator is told of every
         stream that calls ran on, so that it waits for them before it gives that memory to other tensors."""
-        s = self._raw_stream()
+        # the handle alone: torch.cuda.current_stream builds an object around it
+        s = torch._C._cuda_getCurrentRawStream(self._index)
         if s not in self._streams:
             for t in (self._own, self.k_pages, self.v_pages):
                 t.record_stream(torch.cuda.current_stream(self.device))
