@@ -314,7 +314,7 @@ int taco_kv_take_status(const TacoKvPool* pool, int32_t* bits, taco_stream_t str
  *   mass [B, kv_heads, side_ld] fp32, or NULL: 0 for the new slots
  *   positions [B, kv_heads, side_ld] int32, or NULL: first[b] + t (first NULL = starts) for the new slots
  *   lengths_out [B] int32: starts[b] + counts[b]. Not in place: a buffer apart from starts, counts and first (else refused)
- * side_ld >= max_pages * page_size. Tokens beyond the table's capacity are dropped (TACO_KV_BAD_LENGTH). The pages that
+ * side_ld >= max_pages * page_size, T * kv_heads <= 2^25. Tokens beyond the table's capacity are dropped (TACO_KV_BAD_LENGTH). The pages that
  * are written must be the sequence's own, and k and v no part of the pool. */
 int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
                    const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
@@ -327,11 +327,15 @@ int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_l
  *   mass[b][j][t] += sum over the `group` query heads h of kv head j of exp(s[h][t] - lse[b][h])      (mass not NULL)
  * q [B, q_heads, head_dim] by strides of batch and head, q_heads = group * kv_heads; out [B, q_heads, head_dim] and
  * lse [B, q_heads] (fp32, natural log) contiguous and apart from all that is read, but out may be q itself where that is
- * contiguous (another overlap with q is refused); mass [B, kv_heads, side_ld] fp32. Pages may be shared between sequences. A row without tokens, or whose scores are all -inf, gives out 0 and lse -inf and leaves its mass alone.
+ * contiguous (another overlap with q is refused); mass [B, kv_heads, side_ld] fp32. Pages may be shared between sequences.
+ * A row without tokens, or whose scores are all -inf, gives out 0 and lse -inf and leaves its mass alone.
  * What masked slots and unused pages hold (NaN, infinities) has no influence; a NaN or an infinity among a row's own tokens
- * makes that row's output NaN or infinite and no other. Sums and softmax statistics are fp32. The same call gives the same
- * bits; how a row's sums are cut depends on the batch and all its lengths, so a row's last bits may differ in another. Short
- * memories need no workspace; the size is then given as the least there is, 16 bytes. */
+ * makes that row's output NaN or infinite and no other. Sums and softmax statistics are fp32, of weights relative to the greatest:
+ * values past 3.4e38 / tokens (bf16, fp32) overflow them. Weights meet the values in 24 bits (fp16 pools: 22). The same call gives
+ * the same bits; how a row's sums are cut depends on the batch and all its lengths, so a row's last bits may differ in another.
+ * Short memories need no workspace; the size is then given as the least there is, 16 bytes, which stay untouched.
+ * B * kv_heads * (q_heads / kv_heads + slots / 1024) below 2^24, B * kv_heads * slots / 16 (fp32) or / 32, times the passes of 32
+ * query heads a kv head, below 2^30. */
 size_t taco_kv_attend_workspace_bytes(const TacoKvPool* pool, int32_t B, int32_t q_heads, int32_t max_pages,
                                       int32_t with_mass);
 int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
@@ -341,8 +345,8 @@ int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int64_t table_l
 
 /* Every (sequence, kv head) is cut to n = min(lengths[b], budget) tokens: the `recent` newest by position (those above
  * the greatest position - recent; the lower slots, should positions repeat and more than n be such), then the greatest
- * masses; of equal masses the lower slot stays, NaN counts as the greatest. Kept slots below n stay where they are; the empty slots below n take the kept ones from n on, both in
- * ascending order, so no more rows move than have to (one per head when a sequence is one over its budget) and attention,
+ * masses; of equal masses the lower slot stays, NaN counts as the greatest. Tokens that were appended and never attended have
+ * mass 0. Kept slots below n stay where they are; the empty slots below n take the kept ones from n on, both in ascending order, so no more rows move than have to (one per head when a sequence is one over its budget) and attention,
  * which does not depend on the order of slots, goes on. positions says which token a slot holds.
  *   mass, positions [B, kv_heads, side_ld] -> mass_out, positions_out: slots >= n get 0 and -1
  *   lengths_out [B]: n.  Each output may be the matching input itself; no other overlap.

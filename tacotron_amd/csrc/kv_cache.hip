@@ -140,7 +140,8 @@ constexpr int attend_per_cu(int dim) { return dim == 64 ? 2 : 1; }
 
 // Query heads of a group that one pass over K and V serves: 32 where there are more than 16 (32 heads over one of 128, 32 x
 // 8192 tokens, bf16: 32 us in one pass, 39 in two), but at fp32 and D = 256, where two tiles' sums do not fit the registers
-// (124 us against 119).
+// (124 us against 119). 16-bit types at 256 just about do: ten registers go to scratch, and one pass still wins everywhere (32 x
+// 8192 tokens, bf16, weights collected: 84 us against 117 with 32 heads, 71 against 112 with 17; 128 x 512 47 against 50).
 __host__ __device__ constexpr int attend_columns(int dtype, int dim, int group) { return group > 16 && !(dtype == KV_F32 && dim == 256) ? 32 : 16; }
 static int attend_columns(const KvPool& p, int group) { return attend_columns(p.dtype, p.dim, group); }
 static int attend_passes(const KvPool& p, int group) { return (group + attend_columns(p, group) - 1) / attend_columns(p, group); }

@@ -167,7 +167,8 @@ class KvCache:
     def append(self, k, v, page_table, starts, counts=None, first=None, mass=None, positions=None):
         """k, v [B, T, kv_heads, head_dim] -> slots starts[b] .. starts[b] + counts[b] - 1 (counts None: all T) of each
         sequence's pages. mass [B, kv_heads, slots] becomes 0 there, positions [B, kv_heads, slots] first[b] + t (first
-        None: starts). Returns the new lengths, starts + counts. The pages written must belong to one sequence."""
+        None: starts, which after an eviction are not the tokens' own any more). Returns the new lengths, starts + counts.
+        The pages written must belong to one sequence; T * kv_heads is at most 2^25."""
         for name, t in (('k', k), ('v', v)):
             if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[2] != self.kv_heads or t.shape[3] != self.head_dim or not t.numel():
                 raise TacoError('%s must be [B, T, %d, %d]' % (name, self.kv_heads, self.head_dim))
@@ -221,8 +222,8 @@ class KvCache:
         return out, lse
 
     def evict(self, page_table, lengths, mass, positions, budget, recent=0, out=None):
-        """Cuts every (sequence, kv head) to min(lengths[b], budget) tokens: the `recent` newest by position, then those of
-        the greatest mass (ties: the lower slot). Survivors from beyond the budget fill the slots that became empty, so
+        """Cuts every (sequence, kv head) to min(lengths[b], budget) tokens: the newest (positions above the greatest one -
+        `recent`), then those of the greatest mass (ties: the lower slot; a token never attended has 0). Survivors from beyond the budget fill the slots that became empty, so
         slots end up in no order; `positions` tells which token a slot holds. Returns (lengths, mass, positions), new
         tensors, or `out` = three tensors to write, each of which may be the matching input itself. Slots from the new
         length on get mass 0 and position -1 and their pages may be given away. The pages must belong to one sequence."""
