@@ -251,3 +251,67 @@ def test_attend_weights_keep_their_bits(dtype, d, slots):
     tol += np.abs(want) * (torch.finfo(t).eps / 2 + 4 * U) + torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
     assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
     assert (out[:, 0, :5] == 0).all() and (out[:, 0, 6:] == 0).all()
+
+
+@pytest.mark.parametrize('inplace', [False, True])
+@pytest.mark.parametrize('recent', [0, 7])
+def test_evict_one_over_in_a_table_shared_by_workgroups(inplace, recent):
+    """A token over the budget where a head is more than one workgroup holds; masses all different, and all the same."""
+    import torch
+    from tests.test_gpu_kv_cache import _check_evict
+    for same in (False, True):
+        lens = [20001, 300, 0, 20000, 20001]
+        cache, table, lengths = _make(81, lens, 2, 64, 32, 'float16')
+        g = torch.Generator().manual_seed(4)
+        shape = (len(lens), 2, table.shape[1] * 32)
+        mass = torch.full(shape, 0.5) if same else torch.rand(shape, generator=g)
+        pos = torch.stack([torch.randperm(shape[2], generator=g) for _ in range(shape[0] * 2)]).view(shape).to(torch.int32)
+        _check_evict(cache, table, lengths, mass.cuda(), pos.cuda(), 20000, recent, inplace)
+
+
+def test_two_threads_on_one_cache():
+    """Appends, attentions and evictions of two threads, each on a stream of its own, over one pool: the bits of one after the other."""
+    import threading
+
+    import torch
+    lens = [[600, 31, 2], [90, 64, 1200]]
+    cache, table, lengths = _make(91, lens[0] + lens[1], 2, 64, 16, 'bfloat16', slots=1216)
+    own = [(table[3 * i:3 * i + 3], lengths[3 * i:3 * i + 3]) for i in range(2)]
+    pages = [x.clone() for x in (cache.k_pages, cache.v_pages)]
+    qs = [[_q(100 * i + j, 3, 4, 64, 'bfloat16') for j in range(6)] for i in range(2)]
+    sides = torch.rand(3, 2, 1216, generator=torch.Generator().manual_seed(5)).cuda()
+
+    def work(i, out):
+        tab, n = own[i]
+        n, mass = n.clone(), sides.clone()
+        pos = torch.arange(1216, dtype=torch.int32, device='cuda').expand(3, 2, 1216).contiguous()
+        for j in range(6):
+            o, lse = cache.attend(qs[i][j], tab, n, mass=mass)
+            n, mass, pos = cache.evict(tab, n, mass, pos, 500 - 60 * j, 4)
+            n = cache.append(qs[i][j][:, None, :2], qs[i][j][:, None, 2:], tab, n - 1, first=pos.amax((1, 2)) + 1, mass=mass, positions=pos)
+            out += [o, lse, n, mass.clone(), pos.clone()]
+
+    want = [[], []]
+    for i in range(2):
+        work(i, want[i])
+    torch.cuda.synchronize()
+    final = [x.clone() for x in (cache.k_pages, cache.v_pages)]
+    for _ in range(3):
+        for x, y in zip((cache.k_pages, cache.v_pages), pages):
+            x.copy_(y)
+        torch.cuda.synchronize()
+        got, threads = [[], []], []
+        for i in range(2):
+            def run(i=i):
+                with torch.cuda.stream(torch.cuda.Stream()):
+                    work(i, got[i])
+            threads.append(threading.Thread(target=run))
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert len(got[i]) == 30 and all(_same(a, b) for a, b in zip(got[i], want[i]))
+        assert all(_same(a, b) for a, b in zip((cache.k_pages, cache.v_pages), final))
+    cache.status()
