@@ -270,8 +270,8 @@ int taco_debug_conv_gemm(const float* X, int32_t ldx, int32_t M, int32_t T, int3
 /* ---------------------------------------------------------------------------------------
  * Paged key-value cache of an attention decoder (no counterpart in the reference, whose decoder attends one fixed
  * memory per utterance: model/decoder.py:24-27). For decoders whose memories are long, ragged or grow while they decode:
- * a pool of pages shared by all sequences, the attention of ONE new token per sequence over its pages (what taco_decode
- * does once per step over the encoder outputs, as a scaled dot product with any number of query heads per key head), and
+ * a pool of pages shared by all sequences, the attention of ONE new token per sequence over its pages (a scaled dot product with
+ * any number of query heads per key head, where taco_decode attends additively over the encoder outputs and calls none of these), and
  * an eviction that bounds a memory by the attention its tokens have drawn, summed over the steps (the alignments).
  *
  * No model handle: no weights take part. Unlike the calls above, tensors may be strided where a stride is an argument.

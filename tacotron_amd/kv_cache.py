@@ -1,9 +1,9 @@
 """KvCache: a paged key-value cache on one GPU and the three calls that use it (include/taco.h, taco_kv_*): append rows,
 attend one new token per sequence, evict by the attention tokens have drawn.
 
-For decoders whose attention memories are long, ragged or grow while they decode; the encoder memory of one utterance
-(`TacoEngine.encode`, [T_in, 256]) is the simplest case: one kv head of dim 256, appended once, attended every step, the
-collected `mass` being the alignments summed over the steps.
+For decoders with dot-product attention over memories that are long, ragged or grow while they decode; the encoder memory of one
+utterance (`TacoEngine.encode`, [T_in, 256]) is the simplest case: one kv head of dim 256, appended once, attended every step, the
+collected `mass` being the alignments summed over the steps. (The Tacotron decoder itself attends additively and does not come here.)
 
 The cache object holds the pool's geometry and a status word. Everything else - page tables, lengths, masses, positions -
 is the caller's and is passed to each call, so one pool serves any number of batches and a captured HIP graph follows what
