@@ -1807,7 +1807,7 @@ extern "C" int taco_kv_attend(const TacoKvPool* pool, const int32_t* table, int6
     // Queries are read as a wave comes to their head, when other heads may be written already. A head's own row is written by
     // who read it, or after all have: contiguous queries may be written over in place.
     const size_t heads = (size_t)B * q_heads;
-    const bool in_place = out == q && a.q_st[1] == p.dim && (B == 1 || a.q_st[0] == (int64_t)q_heads * p.dim);
+    const bool in_place = out == q && (q_heads == 1 || a.q_st[1] == p.dim) && (B == 1 || a.q_st[0] == (int64_t)q_heads * p.dim);
     if ((!in_place && meets_queries(out, heads * p.dim * p.esize, p, a, B)) || meets_queries(lse, heads * sizeof(float), p, a, B))
         return fail("%s: out must be the (contiguous) queries or not overlap them, nor may lse", what);
     DeviceScope scope(pool->device);

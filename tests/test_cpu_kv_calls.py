@@ -131,3 +131,12 @@ def test_gradients_are_refused_and_not_dropped():
     for k, v in ((pool.clone().requires_grad_(), pool), (pool, pool.clone().requires_grad_())):
         with pytest.raises(TacoError, match='gradient'):
             KvCache(k, v)
+
+
+def test_attend_in_place_of_one_query_head():
+    """One head: its stride says nothing."""
+    from tacotron_amd import _lib
+    args = dict(B=2, q=1 << 20, q_heads=1, out=1 << 20, lse=1 << 22)
+    for qs, refused in (((64, 64), False), ((64, 4096), False), ((128, 64), True)):
+        assert _attend(_lib.load_library(), _pool(device=NOWHERE, kv_heads=1), qs=qs, **args) < 0
+        assert ('overlap' if refused else 'device') in _lib.last_error(), (qs, _lib.last_error())
