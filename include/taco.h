@@ -314,8 +314,8 @@ int taco_kv_take_status(const TacoKvPool* pool, int32_t* bits, taco_stream_t str
  *   mass [B, kv_heads, side_ld] fp32, or NULL: 0 for the new slots
  *   positions [B, kv_heads, side_ld] int32, or NULL: first[b] + t (first NULL = starts) for the new slots
  *   lengths_out [B] int32: starts[b] + counts[b]. Not in place: a buffer apart from starts, counts and first (else refused)
- * side_ld >= max_pages * page_size, T * kv_heads <= 2^25. Tokens beyond the table's capacity are dropped (TACO_KV_BAD_LENGTH). The pages that
- * are written must be the sequence's own, and k and v no part of the pool. */
+ * side_ld >= max_pages * page_size, T * kv_heads <= 2^25. Tokens beyond the table's capacity are dropped
+ * (TACO_KV_BAD_LENGTH). The pages that are written must be the sequence's own, and k and v no part of the pool. */
 int taco_kv_append(const TacoKvPool* pool, const int32_t* table, int64_t table_ld, int32_t B, int32_t max_pages,
                    const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
                    const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride, int32_t T,

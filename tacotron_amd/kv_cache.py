@@ -46,7 +46,7 @@ class KvCache:
         self.device, self.dtype, self._index = k_pages.device, k_pages.dtype, k_pages.device.index
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
         own = torch.zeros(8, dtype=torch.int32, device=self.device)
-        self._own, self._streams = own, {torch._C._cuda_getCurrentRawStream(self._index)}
+        self._own, self._streams = own, set()
         with torch.cuda.device(self.device):
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream().synchronize()      # zeroed before a call of any stream may set a bit
@@ -223,10 +223,11 @@ class KvCache:
 
     def evict(self, page_table, lengths, mass, positions, budget, recent=0, out=None):
         """Cuts every (sequence, kv head) to min(lengths[b], budget) tokens: the newest (positions above the greatest one -
-        `recent`), then those of the greatest mass (ties: the lower slot; a token never attended has 0). Survivors from beyond the budget fill the slots that became empty, so
-        slots end up in no order; `positions` tells which token a slot holds. Returns (lengths, mass, positions), new
-        tensors, or `out` = three tensors to write, each of which may be the matching input itself. Slots from the new
-        length on get mass 0 and position -1 and their pages may be given away. The pages must belong to one sequence."""
+        `recent`), then those of the greatest mass (ties: the lower slot; a token never attended has 0). Survivors from
+        beyond the budget fill the slots that became empty, so slots end up in no order; `positions` tells which token a
+        slot holds. Returns (lengths, mass, positions), new tensors, or `out` = three tensors to write, each of which may
+        be the matching input itself. Slots from the new length on get mass 0 and position -1 and their pages may be given
+        away. The pages must belong to one sequence."""
         table, table_ld, B, max_pages = self._table(page_table)
         lengths = self._ints(lengths, 'lengths', B)
         slots = max_pages * self.page_size

@@ -166,7 +166,7 @@ def test_a_cache_that_goes_while_a_call_runs():
     held = {x.data_ptr() for x in (cache._status, cache.k_pages, cache.v_pages)}
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
-        torch.cuda._sleep(100_000_000)
+        torch.cuda._sleep(400_000_000)
         out, lse = cache.attend(q, table, lengths)
     del cache
     others = [torch.empty(n, dtype=torch.int32, device='cuda') for n in [8] * 200 + [1 << 20] * 4]
@@ -315,3 +315,24 @@ def test_two_threads_on_one_cache():
             assert len(got[i]) == 30 and all(_same(a, b) for a, b in zip(got[i], want[i]))
         assert all(_same(a, b) for a, b in zip((cache.k_pages, cache.v_pages), final))
     cache.status()
+
+
+def test_a_pool_of_another_stream_that_goes_while_a_call_runs():
+    """A pool made on one stream, its cache made and called on another: neither is given away before that call is over."""
+    import torch
+    from tacotron_amd.kv_cache import KvCache
+    table = torch.zeros(1, 3, dtype=torch.int32, device='cuda')
+    lengths = torch.full((1,), 40, dtype=torch.int32, device='cuda')
+    q = _q(1, 1, 2, 64, 'float32')
+    side = torch.cuda.Stream()
+    pool = [torch.empty(1024, 1, 16, 64, device='cuda') for _ in range(2)]
+    held = {x.data_ptr() for x in pool}
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        cache = KvCache(*pool)
+        torch.cuda._sleep(400_000_000)
+        out, lse = cache.attend(q, table, lengths)
+    del cache, pool
+    others = [torch.empty(1 << 20, dtype=torch.int32, device='cuda') for _ in range(4)]
+    assert not side.query() and not held & {x.data_ptr() for x in others}
+    torch.cuda.synchronize()
